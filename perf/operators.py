@@ -66,7 +66,7 @@ def draw(rng):
     if rng.random() < 0.5:
         vocab += -vocab % 64
     rows = _log_uniform(rng, 1, 8192)
-    while rows * vocab > 500_000_000:
+    while rows * vocab > (200_000_000 if op == "score" else 500_000_000):
         rows //= 2
     case = {"op": op, "rows": rows, "vocab": vocab, "dtype": dtype}
     if op == "score":
@@ -146,17 +146,16 @@ def prepare(case, seed):
         if case["op"] == "score":
             k = case["top"]
             st["logp"], st["entropy"] = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
-            st["lse"] = torch.empty(n, device="cuda")
+            st["norm"] = torch.empty(n, 2, device="cuda")
             st["top_logp"] = torch.empty(n, k, device="cuda") if k else None
             st["top_ids"] = torch.empty(n, k, device="cuda", dtype=torch.int32) if k else None
             return st
-        z = logits.double() if n * v <= 20_000_000 else logits.float()
-        z = z * case["scale"]
-        lse = torch.logsumexp(z, 1)
-        st["lse"] = lse.float()
-        z -= lse[:, None]
-        p = z.exp()
-        st["entropy"] = -(z.clamp_(min=-1e4) * p).sum(1).float()
+        m = logits.amax(1, keepdim=True)
+        lp = (logits.double() if n * v <= 20_000_000 else logits.float()).sub(m).mul_(case["scale"])
+        log_s = torch.logsumexp(lp, 1, keepdim=True)
+        st["norm"] = torch.cat([m.float(), log_s.float()], 1)
+        lp -= log_s
+        st["entropy"] = -(lp.exp() * lp.clamp_(min=-1e4)).sum(1).float()
         st["grad_logp"], st["grad_entropy"] = normal(n), normal(n).mul_(0.01)
         st["grad"] = torch.empty_like(logits)
         return st
@@ -172,10 +171,11 @@ def prepare(case, seed):
     st["weight"] = torch.rand(n, generator=gen, device="cuda").add_(0.5)
     st["grad"] = torch.empty_like(logits)
     if case["op"] == "distill":
-        st["loss"], st["lse"] = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+        st["loss"], st["norm"] = torch.empty(n, device="cuda"), torch.empty(n, 2, device="cuda")
     else:
-        z = (logits.double() if n * v <= 20_000_000 else logits.float()) / case["temperature"]
-        st["lse"] = torch.logsumexp(z, 1).float()
+        m = logits.amax(1, keepdim=True)
+        u = (logits.double() if n * v <= 20_000_000 else logits.float()).sub(m).div_(case["temperature"])
+        st["norm"] = torch.cat([m.float(), torch.logsumexp(u, 1, keepdim=True).float()], 1)
     return st
 
 
@@ -201,19 +201,19 @@ def _own(st):
     dev, case = _device(), st["case"]
     op = case["op"]
     if op == "score":
-        out = ops.Logprobs(st["logp"], st["entropy"], st["lse"], st["top_logp"], st["top_ids"])
+        out = ops.Logprobs(st["logp"], st["entropy"], st["norm"], st["top_logp"], st["top_ids"])
         ops.token_logprobs(dev, st["logits"], st["targets"], top=case["top"], scale=case["scale"], ignore_index=IGNORE, out=out)
-        return {"logp": out.logp, "entropy": out.entropy, "lse": out.lse, "top_logp": out.top_logp, "top_ids": out.top_ids}
+        return {"logp": out.logp, "entropy": out.entropy, "norm": out.norm, "top_logp": out.top_logp, "top_ids": out.top_ids}
     if op == "score_grad":
-        ops.token_logprobs_backward(dev, st["logits"], st["targets"], st["lse"], st["entropy"], st["grad_logp"], st["grad_entropy"],
+        ops.token_logprobs_backward(dev, st["logits"], st["targets"], st["norm"], st["entropy"], st["grad_logp"], st["grad_entropy"],
                                     scale=case["scale"], ignore_index=IGNORE, out=st["grad"])
         return {"grad": st["grad"]}
     if op == "distill":
-        out = ops.Distilled(st["loss"], st["lse"], st["grad"])
+        out = ops.Distilled(st["loss"], st["norm"], st["grad"])
         ops.distill_loss(dev, st["logits"], st["teacher"], st["ids"], temperature=case["temperature"], row_weight=st["weight"], grad=True, out=out)
-        return {"loss": out.loss, "lse": out.lse, "grad": out.grad}
+        return {"loss": out.loss, "norm": out.norm, "grad": out.grad}
     if op == "distill_grad":
-        ops.distill_loss_backward(dev, st["logits"], st["teacher"], st["ids"], st["lse"], st["weight"], temperature=case["temperature"], out=st["grad"])
+        ops.distill_loss_backward(dev, st["logits"], st["teacher"], st["ids"], st["norm"], st["weight"], temperature=case["temperature"], out=st["grad"])
         return {"grad": st["grad"]}
     if op == "scan":
         ops.gated_scan(dev, st["gate"], st["x"], state=st["state"], lengths=st["lengths"], log_gate=case["log_gate"], out=st["out"], final=st["final"])
@@ -223,22 +223,21 @@ def _own(st):
     return {"grad_gate": st["grad_gate"], "grad_x": st["grad_x"], "grad_state": st["grad_state"]}
 
 
-def _softmax_parts(u):
-    """Row maximum, exp(u - max), its sum and the logarithm of the sum of exponentials."""
-    m = u.amax(1, keepdim=True)
-    e = torch.exp(u - m)
-    s = e.sum(1, keepdim=True)
-    return m, e, s, m + torch.log(s)
+def _softmax_parts(z, scale):
+    """Row maximum m, scale (z - m), its exponentials, and the logarithm of their sum."""
+    m = z.amax(1, keepdim=True)
+    d = (z - m) * scale
+    e = torch.exp(d)
+    return m, d, e, torch.log(e.sum(1, keepdim=True))
 
 
 def _score(st):
     case = st["case"]
     z = st["logits"].float()
-    u = z * case["scale"]
-    m, e, s, lse = _softmax_parts(u)
-    entropy = torch.log(s) - (torch.where(e > 0, u - m, 0.0) * e).sum(1, keepdim=True) / s
+    m, d, e, log_s = _softmax_parts(z, case["scale"])
+    entropy = log_s - (torch.where(e > 0, d, 0.0) * e).sum(1, keepdim=True) / torch.exp(log_s)
     t = st["targets"]
-    logp = torch.where(t != IGNORE, u.gather(1, t.clamp(min=0)[:, None])[:, 0] - lse[:, 0], 0.0)
+    logp = torch.where(t != IGNORE, d.gather(1, t.clamp(min=0)[:, None])[:, 0] - log_s[:, 0], 0.0)
     top_logp = top_ids = None
     if case["top"]:
         # one whole number for each entry, its value above its place counted from the end: equal values go to the lowest place
@@ -247,13 +246,18 @@ def _score(st):
         place = torch.arange(z.shape[1] - 1, -1, -1, device=z.device)
         best = (key * 4294967296 + place).topk(case["top"], 1).indices
         top_ids = best.int()
-        top_logp = u.gather(1, best) - lse
-    return {"logp": logp, "entropy": entropy[:, 0], "lse": lse[:, 0], "top_logp": top_logp, "top_ids": top_ids}
+        top_logp = d.gather(1, best) - log_s
+    return {"logp": logp, "entropy": entropy[:, 0], "norm": torch.cat([m, log_s], 1), "top_logp": top_logp, "top_ids": top_ids}
+
+
+def _log_probabilities(st, scale):
+    m, log_s = st["norm"][:, :1], st["norm"][:, 1:]
+    return (st["logits"].float() - m) * scale - log_s
 
 
 def _score_grad(st):
     case = st["case"]
-    lp = st["logits"].float() * case["scale"] - st["lse"][:, None]
+    lp = _log_probabilities(st, case["scale"])
     p = torch.exp(lp)
     t = st["targets"]
     g = torch.where(t != IGNORE, st["grad_logp"], 0.0)
@@ -276,18 +280,18 @@ def _teacher(st):
 def _distill(st):
     case = st["case"]
     temp, dt = case["temperature"], st["logits"].dtype
-    m, e, s, lse = _softmax_parts(st["logits"].float() / temp)
+    m, d, e, log_s = _softmax_parts(st["logits"].float(), 1.0 / temp)
     q, log_q = _teacher(st)
     ids = st["ids"].clamp(min=0).long()
-    log_p = st["logits"].gather(1, ids).float() / temp - lse
+    log_p = d.gather(1, ids) - log_s
     loss = temp * temp * (torch.where(q > 0, log_q - log_p, 0.0) * q).sum(1)
-    grad = e.mul_(q.sum(1, keepdim=True) / s).scatter_add_(1, ids, -q)
-    return {"loss": loss, "lse": lse[:, 0], "grad": (grad.mul_(temp * st["weight"][:, None])).to(dt)}
+    grad = e.mul_(q.sum(1, keepdim=True) / torch.exp(log_s)).scatter_add_(1, ids, -q)
+    return {"loss": loss, "norm": torch.cat([m, log_s], 1), "grad": (grad.mul_(temp * st["weight"][:, None])).to(dt)}
 
 
 def _distill_grad(st):
     temp, dt = st["case"]["temperature"], st["logits"].dtype
-    p = torch.exp(st["logits"].float() / temp - st["lse"][:, None])
+    p = torch.exp(_log_probabilities(st, 1.0 / temp))
     q, _ = _teacher(st)
     grad = p.mul_(q.sum(1, keepdim=True)).scatter_add_(1, st["ids"].clamp(min=0).long(), -q)
     return {"grad": grad.mul_(temp * st["weight"][:, None]).to(dt)}
@@ -364,10 +368,10 @@ def _exact_rows(case, st, rows):
     z = st["logits"][rows].double()
     v = z.shape[1]
     if case["op"].startswith("score"):
-        u = z * case["scale"]
         t = st["targets"][rows]
         live = t != IGNORE
         if case["op"] == "score":
+            u = z * case["scale"]
             lse = torch.logsumexp(u, 1)
             lp = u - lse[:, None]
             p = torch.exp(lp)
@@ -377,8 +381,10 @@ def _exact_rows(case, st, rows):
             if case["top"]:
                 order = torch.sort(z, dim=1, descending=True, stable=True).indices[:, : case["top"]]
                 top_logp, top_ids = lp.gather(1, order), order.int()
-            return {"logp": logp, "entropy": entropy, "lse": lse, "top_logp": top_logp, "top_ids": top_ids}
-        lp = u - st["lse"][rows].double()[:, None]
+            largest = z.max(1).values
+            return {"logp": logp, "entropy": entropy, "norm": torch.stack([largest, lse - largest * case["scale"]], 1), "top_logp": top_logp, "top_ids": top_ids}
+        norm = st["norm"][rows].double()
+        lp = case["scale"] * (z - norm[:, :1]) - norm[:, 1:]
         p = torch.exp(lp)
         g = torch.where(live, st["grad_logp"][rows].double(), 0.0)[:, None]
         hot = torch.arange(v, device=z.device)[None, :] == t[:, None]
@@ -389,15 +395,19 @@ def _exact_rows(case, st, rows):
     w = st["weight"][rows].double()
     teacher = torch.where(ids >= 0, st["teacher"][rows].double() / temp, -math.inf)
     q = torch.nan_to_num(torch.softmax(teacher, 1), nan=0.0)
-    lse = torch.logsumexp(z / temp, 1) if case["op"] == "distill" else st["lse"][rows].double()
-    log_p = z / temp - lse[:, None]
+    if case["op"] == "distill":
+        largest = z.max(1).values[:, None]
+        log_s = torch.logsumexp((z - largest) / temp, 1, keepdim=True)
+    else:
+        largest, log_s = st["norm"][rows].double().split(1, 1)
+    log_p = (z - largest) / temp - log_s
     spread = torch.zeros_like(z)
     spread.scatter_add_(1, ids.clamp(min=0), q)
     grad = (w * temp)[:, None] * (torch.exp(log_p) * q.sum(1)[:, None] - spread)
     if case["op"] == "distill_grad":
         return {"grad": grad}
     kl = (torch.xlogy(q, q) - q * log_p.gather(1, ids.clamp(min=0))).sum(1)
-    return {"loss": temp * temp * kl, "lse": lse, "grad": grad}
+    return {"loss": temp * temp * kl, "norm": torch.cat([largest, log_s], 1), "grad": grad}
 
 
 def _exact_scan(case, st):
