@@ -55,6 +55,7 @@ _SIGS = {
     "eh_free": ([_P], None),
     "eh_device_count": ([POINTER(c_int)], c_int),
     "eh_device_open": ([c_int, POINTER(_P)], c_int),
+    "eh_device_open_on_stream": ([c_int, _P, POINTER(_P)], c_int),
     "eh_device_close": ([_P], c_int),
     "eh_device_get_props": ([_P, POINTER(DeviceProps)], c_int),
     "eh_device_sync": ([_P], c_int),
@@ -100,6 +101,17 @@ _SIGS = {
     "eh_module_load": ([_P, _P, c_size_t, c_char_p, POINTER(_P)], c_int),
     "eh_module_launch": ([_P, POINTER(c_uint), POINTER(c_uint), c_uint, POINTER(_P), c_int, c_int], c_int),
     "eh_module_release": ([_P], c_int),
+    # (the operators' argument structures travel as packed bytes)
+    "eh_token_logprobs": ([_P, c_char_p, c_int], c_int),
+    "eh_token_logprobs_workspace": ([_P, c_char_p, POINTER(c_size_t)], c_int),
+    "eh_token_logprobs_backward": ([_P, c_char_p, c_int], c_int),
+    "eh_distill_loss": ([_P, c_char_p, c_int], c_int),
+    "eh_distill_loss_workspace": ([_P, c_char_p, POINTER(c_size_t)], c_int),
+    "eh_distill_loss_backward": ([_P, c_char_p, c_int], c_int),
+    "eh_gated_scan": ([_P, c_char_p, c_int], c_int),
+    "eh_gated_scan_workspace": ([_P, c_char_p, POINTER(c_size_t)], c_int),
+    "eh_gated_scan_backward": ([_P, c_char_p, c_int], c_int),
+    "eh_gated_scan_backward_workspace": ([_P, c_char_p, POINTER(c_size_t)], c_int),
     "eh_event_create": ([_P, POINTER(_P)], c_int),
     "eh_event_record": ([_P], c_int),
     "eh_event_sync": ([_P], c_int),

@@ -123,9 +123,15 @@ def device_count() -> int:
 # ---------------------------------------------------------------------------
 
 class HipDevice:
-    def __init__(self, index: int = 0):
+    """A device handle with a stream of its own, or with `stream` (a hipStream_t as an integer, 0 for the
+    device's default stream) on the caller's: its work is then ordered with the caller's on that stream."""
+
+    def __init__(self, index: int = 0, stream: Optional[int] = None):
         self._h = c_void_p()
-        check(lib.eh_device_open(index, byref(self._h)))
+        if stream is None:
+            check(lib.eh_device_open(index, byref(self._h)))
+        else:
+            check(lib.eh_device_open_on_stream(index, c_void_p(stream), byref(self._h)))
         self.index = index
         p = DeviceProps()
         check(lib.eh_device_get_props(self._h, byref(p)))

@@ -18,9 +18,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libeclat_hip.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
-SOURCES = ["ast.cpp", "analysis.cpp", "normalize.cpp", "codegen.cpp", "stages.cpp", "rewrites.cpp", "plan.cpp", "emitters.cpp", "launches.cpp", "gemm.cpp", "window.cpp", "backend.cpp", "capi.cpp"]
-# compiled as HIP for gfx950: holds the library's one statically allocated device array
-DEVICE_SOURCES = ["static_scratch.hip"]
+SOURCES = ["ast.cpp", "analysis.cpp", "normalize.cpp", "codegen.cpp", "stages.cpp", "rewrites.cpp", "plan.cpp", "emitters.cpp", "launches.cpp", "gemm.cpp", "window.cpp", "backend.cpp", "capi.cpp", "operators.cpp"]
+# compiled as HIP for gfx950: the library's one statically allocated device array and the kernels that
+# are compiled ahead of time
+DEVICE_SOURCES = ["static_scratch.hip", "kernels/token_rows.hip", "kernels/gated_scan.hip"]
 TEMPLATES = ["kernels/gemm_f32_mfma.hip", "kernels/window_f32_mfma.hip"]
 DEVICE_FLAGS = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off",
                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -62,7 +63,8 @@ def build(check: bool = False, force: bool = True) -> str:
     srcs = [os.path.join(CSRC, s) for s in SOURCES + DEVICE_SOURCES]
     if not force and os.path.exists(LIB):
         newest = max(os.path.getmtime(p) for p in srcs + [os.path.join(CSRC, t) for t in TEMPLATES]
-                     + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".hpp")])
+                     + [os.path.join(d, h) for d in (CSRC, os.path.join(CSRC, "kernels")) for h in os.listdir(d)
+                        if h.endswith(".hpp")])
         if os.path.getmtime(LIB) >= newest:
             return LIB
     hipcc = os.path.join(ROCM, "bin", "hipcc")
@@ -72,7 +74,7 @@ def build(check: bool = False, force: bool = True) -> str:
         for s in srcs:
             o = os.path.join(tmp, os.path.basename(s) + ".o")
             objs.append(o)
-            if os.path.basename(s) in DEVICE_SOURCES:
+            if s.endswith(".hip"):
                 cmd = [hipcc, "-std=c++17", "-fPIC", "-Wall", "-Wextra"] + DEVICE_FLAGS + ["-c", s, "-o", o]
             else:
                 cmd = [hipcc, "-x", "c++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Wextra",

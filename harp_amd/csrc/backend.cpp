@@ -194,6 +194,19 @@ int HipDevice::count() {
 }
 
 HipDevice::HipDevice(int index) : index_(index) {
+  open();
+  check(hipStreamCreate(&stream_), "hipStreamCreate");
+  owns_stream_ = true;
+  opened_ = true;
+}
+
+HipDevice::HipDevice(int index, hipStream_t stream) : index_(index), stream_(stream) {
+  open();
+  opened_ = true;
+}
+
+void HipDevice::open() {
+  const int index = index_;
   int n = count();
   if (n == 0) throw Error("no HIP device is present (hipGetDeviceCount found none)");
   if (index < 0 || index >= n)
@@ -213,7 +226,6 @@ HipDevice::HipDevice(int index) : index_(index) {
   profile_.memory_clock_khz = p.memoryClockRate;
   profile_.memory_bus_bits = p.memoryBusWidth;
   profile_.l2_bytes = p.l2CacheSize;
-  check(hipStreamCreate(&stream_), "hipStreamCreate");
   pool_limit_ = std::getenv("ECLAT_HIP_NO_POOL") ? 0 : profile_.global_memory_size / 4;
   // resolved here, with this device current, so that the entry point which must not allocate
   // never triggers the load of the library's code object itself
@@ -230,7 +242,7 @@ void* HipDevice::static_scratch() const {
 }
 
 HipDevice::~HipDevice() {
-  if (stream_) {
+  if (opened_) {
     (void)hipSetDevice(index_);
     (void)hipStreamSynchronize(stream_);
     for (hipStream_t st : side_streams_) {
@@ -238,7 +250,7 @@ HipDevice::~HipDevice() {
       (void)hipStreamDestroy(st);
     }
     for (auto& kv : pool_) (void)hipFree(kv.second);
-    (void)hipStreamDestroy(stream_);
+    if (owns_stream_) (void)hipStreamDestroy(stream_);
   }
 }
 

@@ -51,6 +51,7 @@ class HipDevice {
   static int count();                  // 0 when no GPU/driver is present
   static bool is_available() { return count() > 0; }
   explicit HipDevice(int index);
+  HipDevice(int index, hipStream_t stream);   // queues on the caller's stream, which it does not own
   ~HipDevice();
   HipDevice(const HipDevice&) = delete;
   HipDevice& operator=(const HipDevice&) = delete;
@@ -88,8 +89,11 @@ class HipDevice {
   void* static_scratch() const;
 
  private:
+  void open();
   int index_;
   hipStream_t stream_ = nullptr;
+  bool owns_stream_ = false;
+  bool opened_ = false;
   std::vector<hipStream_t> side_streams_;
   DeviceProfile profile_;
   mutable std::recursive_mutex stream_mu_;

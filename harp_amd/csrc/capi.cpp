@@ -9,19 +9,12 @@
 
 #include "../../include/eclat_hip.h"
 #include "backend.hpp"
+#include "handles.hpp"
 #include "normalize.hpp"
 #include "static_scratch.hpp"
 
 using namespace eh;
 
-struct eh_device {
-  HipDevice dev;
-  explicit eh_device(int i) : dev(i) {}
-};
-struct eh_buffer {
-  HipBuffer buf;
-  eh_buffer(HipDevice* d, size_t n) : buf(d, n) {}
-};
 struct eh_program {
   HipProgram prog;
   eh_program(HipDevice* d, const std::string& t, const GenOptions& o) : prog(d, t, o) {}
@@ -51,6 +44,10 @@ namespace {
 
 thread_local std::string g_err;
 
+}  // namespace
+
+namespace eh {
+
 int fail(int code, const std::string& msg) {
   g_err = msg;
   return code;
@@ -68,18 +65,9 @@ int classify(const std::string& m) {
   return EH_ERR_INVALID;
 }
 
-template <class F> int guard(F&& f) {
-  try {
-    f();
-    return EH_OK;
-  } catch (const Error& e) {
-    return fail(classify(e.what()), e.what());
-  } catch (const std::bad_alloc&) {
-    return fail(EH_ERR_INVALID, "out of host memory");
-  } catch (const std::exception& e) {
-    return fail(EH_ERR_INVALID, e.what());
-  }
-}
+}  // namespace eh
+
+namespace {
 
 void fill_info(const LaunchSpec& ls, eh_launch_info* out) {
   out->entry = ls.entry.c_str();
@@ -129,6 +117,16 @@ int eh_device_count(int* count) {
 int eh_device_open(int index, eh_device** out) {
   REQUIRE(out, "out is NULL");
   return guard([&] { *out = new eh_device(index); });
+}
+
+int eh_device_open_on_stream(int index, void* stream, eh_device** out) {
+  REQUIRE(out, "out is NULL");
+  return guard([&] {
+    int current = -1;
+    if (hipGetDevice(&current) != hipSuccess) (void)hipGetLastError();
+    *out = new eh_device(index, static_cast<hipStream_t>(stream));
+    if (current >= 0 && current != index) (void)hipSetDevice(current);
+  });
 }
 
 int eh_device_close(eh_device* dev) {

@@ -1,0 +1,114 @@
+// The language-model operators' kernels as the entry points (operators.cpp) see them: plain
+// structures of device addresses and sizes, already checked, and one launch function each.
+#pragma once
+
+#include <hip/hip_runtime_api.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace eh {
+
+enum ElemType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+inline size_t elem_size(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+constexpr int kMaxTop = 32;          // alternatives a row can report: one wave selects them among 64 groups
+constexpr int kMaxTeacher = 1024;    // entries a teacher can give for a row: they are held in LDS
+
+// Rows of logits: element (r, i) at z + (r * stride + i) elements.
+struct LogitRows {
+  const void* z;
+  int64_t stride;
+  int64_t rows;
+  int vocab;
+  int dtype;
+  float scale;             // 1 / temperature
+};
+
+struct TokenIds {
+  const void* ids;
+  int wide;                // 64-bit integers
+};
+
+// One row's share of work for a workgroup: `segs` segments of `seg` elements.
+struct RowSplit {
+  int segs;
+  int seg;
+};
+// Splits rows until the launch fills the device; a whole row (segs == 1) where there are enough.
+RowSplit split_rows(int64_t rows, int vocab, int dtype, int compute_units);
+size_t split_workspace(const RowSplit& s, int64_t rows, int top);   // bytes; 0 for whole rows
+
+struct ScoreArgs {
+  LogitRows in;
+  TokenIds targets;
+  int64_t ignore;
+  float* logp;             // [rows]
+  float* entropy;          // [rows] or null
+  float* norm;             // [rows][2]: largest logit, log sum exp(scale (z - largest))
+  float* top_logp;         // [rows][top]
+  int* top_ids;
+  int top;
+  RowSplit split;
+  void* workspace;
+};
+hipError_t launch_score(const ScoreArgs& a, hipStream_t stream);
+
+struct ScoreGradArgs {
+  LogitRows in;
+  TokenIds targets;
+  int64_t ignore;
+  const float* norm;
+  const float* entropy;        // null: no entropy gradient
+  const float* grad_logp;      // null: none
+  const float* grad_entropy;
+  void* grad;
+  int64_t grad_stride;
+};
+hipError_t launch_score_grad(const ScoreGradArgs& a, int compute_units, hipStream_t stream);
+
+struct DistillArgs {
+  LogitRows in;                // scale is 1 / temperature
+  float temperature;
+  const void* teacher;         // [rows][k], element type teacher_dtype
+  int64_t teacher_stride;
+  int teacher_dtype;
+  TokenIds ids;                // [rows][k]
+  int64_t ids_stride;
+  int k;
+  const float* weight;         // [rows] or null: what each row's gradient is multiplied by
+  float* norm;                 // [rows][2]: written by the loss, read by the gradient alone
+  float* loss;                 // [rows]
+  void* grad;                  // null: no gradient
+  int64_t grad_stride;
+  RowSplit split;
+  void* workspace;
+};
+hipError_t launch_distill(const DistillArgs& a, int compute_units, hipStream_t stream);
+hipError_t launch_distill_grad(const DistillArgs& a, int compute_units, hipStream_t stream);
+
+// Element (b, t, d) at p + b * batch + t * step + d elements.
+struct Sequences {
+  void* p;
+  int64_t batch, step;
+};
+
+struct ScanArgs {
+  int64_t batch, time;
+  int width;
+  int dtype;
+  int log_gate;                // gates are exp(gate)
+  Sequences gate, x, out;      // gradients: gate, h (x) and grad_h (out) are read
+  Sequences grad_gate, grad_x; // (gradients only)
+  const float* state;          // [batch][width] or null (zeros)
+  float* final_state;          // [batch][width] or null; gradients: the gradient of `state`
+  const float* grad_final;     // gradients only, or null
+  const int* lengths;          // [batch] or null
+  void* workspace;
+};
+size_t scan_workspace(const ScanArgs& a, int compute_units);
+hipError_t launch_scan(const ScanArgs& a, int compute_units, hipStream_t stream);
+hipError_t launch_scan_grad(const ScanArgs& a, int compute_units, hipStream_t stream);
+
+}  // namespace eh

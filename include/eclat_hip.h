@@ -61,6 +61,11 @@ typedef struct eh_device_props {
 
 int eh_device_count(int* count);        /* 0 devices is not an error */
 int eh_device_open(int index, eh_device** out);
+/* A device handle that queues everything on the caller's stream (a hipStream_t; NULL is the device's
+ * default stream) instead of one of its own: what the library launches is then ordered with the
+ * caller's work on that stream.  The stream must outlive the handle; the calling thread's current
+ * device is left as it was.  Several handles may share a stream. */
+int eh_device_open_on_stream(int index, void* stream, eh_device** out);
 int eh_device_close(eh_device* dev);    /* buffers and programs of the device must be gone */
 int eh_device_get_props(eh_device* dev, eh_device_props* out);
 int eh_device_sync(eh_device* dev);     /* waits for everything queued on the device's stream */
@@ -250,6 +255,120 @@ int eh_module_load(eh_device* dev, const void* blob, size_t len, const char* ent
 int eh_module_launch(eh_module* mod, const unsigned grid[3], const unsigned block[3], unsigned lds_bytes,
                      eh_buffer* const* args, int n_args, int sync);
 int eh_module_release(eh_module* mod);
+
+/* ---- language-model operators ---------------------------------------------------------------------
+ * Hand-written kernels next to what programs render: scores of tokens under rows of logits (beside
+ * log_softmax and cross_entropy_loss, crates/nn/src/functional/activation.rs:174-187, loss.rs:32-65),
+ * distillation from a teacher's top logits, and the gated linear recurrence (beside the scans of
+ * src/lowerer/lower.rs:691-735).  The reference has no counterpart of them.
+ *
+ * All calls queue on the device handle's stream, allocate nothing but a workspace where one is
+ * needed, and may be captured into a graph (give the workspace then).  sync != 0 waits for
+ * completion.  Sums, softmax statistics and states are f32 whatever the arrays' type; every result is
+ * rounded once, to nearest even.  The same inputs give the same bits every time.
+ *
+ * An array is part of a buffer of the library or device memory of the caller's.  Rows and steps
+ * may be apart by any stride; the innermost axis is contiguous.  Sizes are checked against the
+ * buffer (EH_ERR_SIZE).  An output overlaps nothing else of the call, except that arrays of the same
+ * row strides may lie side by side in each other's gaps; its own elements must not overlap.  */
+#define EH_F32 0
+#define EH_BF16 1
+#define EH_F16 2
+#define EH_I32 3
+#define EH_I64 4
+typedef struct eh_array {
+  eh_buffer* buffer;       /* NULL: device memory of the caller's */
+  uint64_t offset;         /* bytes into the buffer; without a buffer the device address.  Both 0: no array */
+  uint64_t bytes;          /* without a buffer: how many bytes are there */
+  int64_t stride[2];       /* elements from row to row; of sequences: from sequence to sequence, from step to step */
+  int64_t dtype;           /* EH_F32 ... */
+} eh_array;
+
+/* Log probabilities under p = softmax(scale * logits) of one given token a row, the entropy, and the
+ * `top` likeliest tokens.
+ *   logits     [rows][vocab]  f32, bf16 or f16; -infinity is a token that cannot occur
+ *   targets    [rows]         i32 or i64.  ignore_index: no token, its log probability is 0.  Any other id
+ *                             outside [0, vocab): NaN
+ *   logp       [rows] f32;    entropy [rows] f32 or absent
+ *   norm       [rows][2] f32  the row's largest logit m and log sum exp(scale * (z - m)): what the
+ *                             gradient reads (log sum exp(scale * z) is scale * m + the second)
+ *   top_logp   [rows][top] f32, top_ids [rows][top] i32 (absent if top == 0; top <= 32 and <= vocab):
+ *                             largest first, equal logits by id (-0 equals 0)
+ * A row without a token above -infinity: logp and top_logp -infinity, entropy 0.  A row with NaN or
+ * +infinity: NaN throughout, the ids are still those of the largest logits that are numbers (-1 where
+ * there are too few).  Small arrays are contiguous.  workspace: see eh_token_logprobs_workspace. */
+typedef struct eh_token_logprobs_args {
+  int64_t rows, vocab, top;
+  int64_t ignore_index;
+  double scale;
+  eh_array logits, targets, logp, entropy, norm, top_logp, top_ids, workspace;
+} eh_token_logprobs_args;
+int eh_token_logprobs(eh_device* dev, const eh_token_logprobs_args* args, int sync);
+/* Bytes of device memory that the call needs besides its arrays: 0 where a row is a workgroup's
+ * work, partial sums where few long rows are split.  Without a `workspace` array the call takes them
+ * from the device's pool; under stream capture it must be given, and graphs whose replays may
+ * overlap need one each. */
+int eh_token_logprobs_workspace(eh_device* dev, const eh_token_logprobs_args* args, size_t* bytes);
+
+/* The gradient with respect to the logits of sum_r (grad_logp_r logp_r + grad_entropy_r entropy_r):
+ *   scale * (g ([i = target] - p_i) - e p_i (log p_i + entropy)).
+ * norm and (with grad_entropy) entropy are those of the call above; grad_logp or grad_entropy may be
+ * absent.  The alternatives have no gradient.  grad: [rows][vocab], of the logits' type. */
+typedef struct eh_token_logprobs_backward_args {
+  int64_t rows, vocab;
+  int64_t ignore_index;
+  double scale;
+  eh_array logits, targets, norm, entropy, grad_logp, grad_entropy, grad;
+} eh_token_logprobs_backward_args;
+int eh_token_logprobs_backward(eh_device* dev, const eh_token_logprobs_backward_args* args, int sync);
+
+/* Distillation from a teacher's top logits: loss_r = T^2 KL(q_r || p_r) with T the temperature,
+ * p = softmax(logits / T) over the vocabulary and q = softmax(teacher / T) over the k tokens that the
+ * teacher names in that row (k <= 1024).
+ *   teacher    [rows][k]      f32, bf16 or f16 logits, any order; ids [rows][k] i32 or i64.  An id outside
+ *                             [0, vocab) is no entry; a token named twice counts twice.  A row without
+ *                             entries has loss 0 and gradient 0
+ *   loss       [rows] f32, norm [rows][2] f32 (as above, with scale 1 / T)
+ *   grad       [rows][vocab] of the logits' type, or absent: weight_r times the gradient of loss_r,
+ *                             weight_r T (p_i - sum of q over the entries that name i)
+ *   weight     [rows] f32, or absent (1)
+ * A row without a logit above -infinity: loss +infinity (0 without teacher entries), gradient 0. */
+typedef struct eh_distill_loss_args {
+  int64_t rows, vocab, k;
+  double temperature;
+  eh_array logits, teacher, ids, weight, loss, norm, grad, workspace;
+} eh_distill_loss_args;
+int eh_distill_loss(eh_device* dev, const eh_distill_loss_args* args, int sync);
+int eh_distill_loss_workspace(eh_device* dev, const eh_distill_loss_args* args, size_t* bytes);
+/* The gradient alone, for upstream gradients `weight` that are known only later: reads norm, takes no
+ * loss and no workspace. */
+int eh_distill_loss_backward(eh_device* dev, const eh_distill_loss_args* args, int sync);
+
+/* The gated linear recurrence h_t = a_t h_(t-1) + x_t for each of `width` channels of `batch`
+ * sequences of up to `time` steps; a = gate, or exp(gate) with log_gate != 0.
+ *   gate, x, out     [batch][time][width], one type of f32, bf16, f16
+ *   state            [batch][width] f32, contiguous, or absent: h_(-1) (0)
+ *   final_state      [batch][width] f32, or absent: h of each sequence's last step (its state, if it has no steps)
+ *   lengths          [batch] i32, or absent: the steps a sequence has (negative: 0, above time: time); what lies
+ *                    behind them is neither read nor written in any array
+ * Products of gates are formed along a sequence, so gates are meant to be at most about 1 in magnitude: a
+ * product that leaves f32's range gives what inf and 0 give. */
+typedef struct eh_gated_scan_args {
+  int64_t batch, time, width, log_gate;
+  eh_array gate, x, state, lengths, out, final_state, workspace;
+} eh_gated_scan_args;
+int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync);
+int eh_gated_scan_workspace(eh_device* dev, const eh_gated_scan_args* args, size_t* bytes);
+/* Its gradients, from the gates, the outputs h of the forward call and grad_h:
+ *   l_t = grad_h_t + a_(t+1) l_(t+1) (with grad_final added at a sequence's last step);
+ *   grad_x = l, grad_gate_t = l_t h_(t-1) (times a_t with log_gate), grad_state = a_0 l_0.
+ * state, lengths, grad_final and grad_state may be absent. */
+typedef struct eh_gated_scan_backward_args {
+  int64_t batch, time, width, log_gate;
+  eh_array gate, h, grad_h, state, lengths, grad_final, grad_gate, grad_x, grad_state, workspace;
+} eh_gated_scan_backward_args;
+int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* args, int sync);
+int eh_gated_scan_backward_workspace(eh_device* dev, const eh_gated_scan_backward_args* args, size_t* bytes);
 
 /* ---- timing on the device's stream (HIP events) ------------------------------------------------ */
 int eh_event_create(eh_device* dev, eh_event** out);
