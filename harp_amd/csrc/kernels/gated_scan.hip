@@ -1,53 +1,303 @@
 // The gated linear recurrence h_t = a_t h_(t-1) + x_t over [batch, time, width], and its gradients.
+//
+// A run of steps maps the state before it to the state behind it, h -> A h + B, and two runs one after
+// the other are (A2 A1, A2 B1 + B2).  The backward pass is the same recurrence in reverse order on
+// c_t = a_t (g_t + c_(t+1)), what step t hands to step t - 1: its steps are the maps (a_t, a_t g_t), and
+//   lambda_t = g_t + c_(t+1),  dx_t = lambda_t,  da_t = lambda_t h_(t-1),  d(log a_t) = da_t a_t,  dh_0 = c_0.
 #include "elements.hpp"
 
 namespace eh {
 namespace {
 
-template <int DT> __device__ inline float at(const Sequences& s, int64_t b, int64_t t, int d) {
-  return Elem<DT>::get(static_cast<const typename Elem<DT>::T*>(s.p)[b * s.batch + t * s.step + d]);
-}
-template <int DT> __device__ inline void put(const Sequences& s, int64_t b, int64_t t, int d, float v) {
-  static_cast<typename Elem<DT>::T*>(s.p)[b * s.batch + t * s.step + d] = Elem<DT>::put(v);
+constexpr int kSteps = 8;            // a thread's own steps, held in registers from the only reading
+constexpr int kLanes = 8;            // lanes side by side: 128 bytes of a step, a whole cache line
+
+template <int DT> struct Chunk {
+  static constexpr int N = Elem<DT>::N;
+  static constexpr int CW = kLanes * N;                                  // channels of a workgroup
+};
+
+// Where a workgroup leaves what later pieces of the same channels need: 64-bit words (A, B) of its own
+// steps, then 32-bit words of the state behind them.  A word says by itself that it is there: nothing
+// writes the all-ones pattern that the words start with, which is one of NaN's.
+struct Board {
+  unsigned int* ticket;
+  unsigned long long* maps;
+  unsigned int* states;
+};
+constexpr unsigned int kEmpty = 0xffffffffu;
+constexpr size_t kTicketBytes = 256;
+
+__device__ inline unsigned int word_of(float x) {
+  const unsigned int b = __float_as_uint(x);
+  return b == kEmpty ? 0x7fc00000u : b;
 }
 
-// A thread for each channel of each sequence, step by step.
-template <int DT> __global__ __launch_bounds__(64) void scan_steps(ScanArgs a) {
-  const int blocks = (a.width + 63) / 64;
-  const int64_t b = blockIdx.x / blocks;
-  const int d = static_cast<int>(blockIdx.x % blocks) * 64 + static_cast<int>(threadIdx.x);
-  if (d >= a.width) return;
-  int64_t n = a.time;
-  if (a.lengths) n = min(n, max(static_cast<int64_t>(a.lengths[b]), int64_t{0}));
-  float h = a.state ? a.state[b * a.width + d] : 0.f;
-  for (int64_t t = 0; t < n; ++t) {
-    float g = at<DT>(a.gate, b, t, d);
-    if (a.log_gate) g = exp2_hw(g * kLog2e);
-    h = __builtin_fmaf(g, h, at<DT>(a.x, b, t, d));
-    put<DT>(a.out, b, t, d, h);
+// Up to N channels of one step; those behind the row's end are 0.
+template <int DT> __device__ inline u32x4 load_some(const typename Elem<DT>::T* p, int n) {
+  constexpr int N = Elem<DT>::N;
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (j >= n) break;
+    if constexpr (N == 4) v[j] = __float_as_uint(p[j]);
+    else v[j / 2] |= static_cast<uint32_t>(p[j]) << (16 * (j % 2));
   }
-  if (a.final_state) a.final_state[b * a.width + d] = h;
+  return v;
+}
+// The rows of a piece, from an address that is the same for the whole workgroup; its rows are within
+// 4 GiB of it unless FAR, so that an address is one register per thread.
+template <int DT, bool FAR> struct PieceRows {
+  char* base;
+  int64_t step;                  // bytes
+  __device__ PieceRows(const Sequences& s, int64_t b, int64_t t, int tile) {
+    constexpr int64_t size = sizeof(typename Elem<DT>::T);
+    base = static_cast<char*>(s.p) + (b * s.batch + t * s.step + tile) * size;
+    step = s.step * size;
+  }
+  __device__ typename Elem<DT>::T* at(int row, uint32_t channel_bytes) const {
+    if constexpr (FAR) return reinterpret_cast<typename Elem<DT>::T*>(base + row * step + channel_bytes);
+    else return reinterpret_cast<typename Elem<DT>::T*>(base + (static_cast<uint32_t>(row) * static_cast<uint32_t>(step) + channel_bytes));
+  }
+};
+
+// kSteps rows from `row` on, each held inside [0, most].
+template <int DT, bool FAR> __device__ inline void load_steps(const PieceRows<DT, FAR>& s, int row, int most, uint32_t cb, int nc, u32x4* v) {
+  if (nc >= Elem<DT>::N) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) v[i] = load16(s.at(max(min(row + i, most), 0), cb));
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < kSteps; ++i) {
+      const u32x4 x = load_some<DT>(s.at(max(min(row + i, most), 0), cb), nc);
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) v[k] = k == i ? x : v[k];
+    }
+  }
+}
+template <int DT> __device__ inline void store_channels(typename Elem<DT>::T* p, int n, const float* z) {
+  constexpr int N = Elem<DT>::N;
+  if (n >= N) {
+    store16(p, Elem<DT>::pack(z));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < n) p[j] = Elem<DT>::put(z[j]);
 }
 
-// lambda_t = g_t + a_(t+1) lambda_(t+1);  dx_t = lambda_t, da_t = lambda_t h_(t-1), d(log a_t) = da_t a_t.
-template <int DT> __global__ __launch_bounds__(64) void scan_grad_steps(ScanArgs a) {
-  const int blocks = (a.width + 63) / 64;
-  const int64_t b = blockIdx.x / blocks;
-  const int d = static_cast<int>(blockIdx.x % blocks) * 64 + static_cast<int>(threadIdx.x);
-  if (d >= a.width) return;
+// The gates and the added values of a step; behind a sequence's end the step changes nothing.
+template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, bool live, float* a, float* x) {
+  constexpr int N = Elem<DT>::N;
+  Elem<DT>::unpack(vg, a);
+  Elem<DT>::unpack(vx, x);
+  if (LOG) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) a[j] = exp2_hw(a[j] * kLog2e);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    a[j] = live ? a[j] : 1.f;
+    x[j] = live ? x[j] : 0.f;
+  }
+}
+
+// A workgroup of W waves has CW channels of W * 64 steps, its piece: eight lanes side by side for the
+// channels, eight runs of kSteps steps one after the other in each wave, the waves one after the
+// other.  Gates and inputs are read once and stay in registers.  Each thread's map, then scans over the
+// lanes, the waves and the pieces of the same channels give the state before each thread's steps, and
+// the steps are run from there.
+//
+// Over the pieces (W == 8; shorter sequences have one): they form groups of P in the order of the
+// steps.  Each leaves its map on the board before it looks at anybody else's, the last of a group the
+// state behind it; a piece composes the state before its group with the maps of the group's pieces
+// before it, all read at once.  Which words are read depends on the piece alone, so results do not
+// depend on the order in which workgroups run.  Workgroups take their pieces from a ticket in the
+// order of the steps: a piece only waits for pieces that have started, for maps that are left without
+// waiting and for the state of the group before, whose waits end for the same reason.
+template <int DT, int W, bool BACK, bool LOG, bool FAR, int EU>
+__global__ __launch_bounds__(64 * W, EU) void scan_chunks(ScanArgs a, int chunks, int tiles, Board board) {
+  constexpr int N = Elem<DT>::N, CW = Chunk<DT>::CW, RUN = W * 64 / kLanes * kSteps, P = 64 * W / CW;
+  typedef typename Elem<DT>::T T;
+  __shared__ float maps[2][W][CW];
+  __shared__ float others[2][P][CW];
+  __shared__ float before[CW];
+  __shared__ unsigned int turn;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t columns = a.batch * tiles;
+  int64_t piece = blockIdx.x;
+  if (W == 8 && chunks > 1) {
+    if (threadIdx.x == 0) turn = atomicAdd(board.ticket, 1u) + 1u;       // the word starts at all ones
+    __syncthreads();
+    piece = turn;
+  }
+  const int64_t column = piece % columns;
+  const int64_t b = column / tiles;
+  const int tile = static_cast<int>(column % tiles) * CW;
+  const int c0 = tile + (lane % kLanes) * N;
+  const int nc = a.width - c0;                                            // channels of this thread (above N: N; below 1: none)
   int64_t n = a.time;
   if (a.lengths) n = min(n, max(static_cast<int64_t>(a.lengths[b]), int64_t{0}));
-  float carry = a.grad_final ? a.grad_final[b * a.width + d] : 0.f;        // a_(t+1) lambda_(t+1)
-  for (int64_t t = n; t-- > 0;) {
-    float g = at<DT>(a.gate, b, t, d);
-    if (a.log_gate) g = exp2_hw(g * kLog2e);
-    const float l = at<DT>(a.out, b, t, d) + carry;
-    const float before = t ? at<DT>(a.x, b, t - 1, d) : a.state ? a.state[b * a.width + d] : 0.f;
-    put<DT>(a.grad_x, b, t, d, l);
-    put<DT>(a.grad_gate, b, t, d, a.log_gate ? l * before * g : l * before);
-    carry = g * l;
+  const int64_t last = n > 0 ? (n - 1) / RUN : 0;                         // the sequence's last piece
+  const int64_t k = BACK ? chunks - 1 - piece / columns : piece / columns;
+  if (k > last) return;
+  const int64_t behind = BACK ? last - k : k;                             // pieces before this one, in the order of the steps
+  const int run = wave * (64 / kLanes) + lane / kLanes;                   // this thread's place among the runs
+  // counted from the piece's first row: this thread's first row, and how many rows the sequence has from there on
+  const int row = (BACK ? W * (64 / kLanes) - 1 - run : run) * kSteps, rows = static_cast<int>(min(n - k * RUN, int64_t{RUN}));
+  const uint32_t cb = static_cast<uint32_t>((lane % kLanes) * N * sizeof(T));
+
+  u32x4 vg[kSteps] = {}, vx[kSteps] = {};
+  if (n > 0 && nc > 0) {
+    load_steps<DT, FAR>({a.gate, b, k * RUN, tile}, row, rows - 1, cb, nc, vg);
+    load_steps<DT, FAR>({BACK ? a.out : a.x, b, k * RUN, tile}, row, rows - 1, cb, nc, vx);
   }
-  if (a.final_state) a.final_state[b * a.width + d] = carry;
+  float A[N], B[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) A[j] = 1.f, B[j] = 0.f;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int i = BACK ? kSteps - 1 - s : s;
+    float g[N], x[N];
+    step_of<DT, LOG>(vg[i], vx[i], row + i < rows, g, x);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      B[j] = BACK ? g[j] * (B[j] + x[j]) : __builtin_fmaf(g[j], B[j], x[j]);
+      A[j] *= g[j];
+    }
+  }
+  // the second run over the steps unpacks them again: kept unpacked they would not fit the registers
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    asm volatile("" : "+v"(vg[i]), "+v"(vx[i]));
+#pragma unroll
+  for (int off = kLanes; off < 64; off *= 2) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float pa = __shfl_up(A[j], off), pb = __shfl_up(B[j], off);
+      if (lane >= off) {
+        B[j] = __builtin_fmaf(A[j], pb, B[j]);
+        A[j] *= pa;
+      }
+    }
+  }
+  if (lane >= 64 - kLanes) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      maps[0][wave][(lane % kLanes) * N + j] = A[j];
+      maps[1][wave][(lane % kLanes) * N + j] = B[j];
+    }
+  }
+  // the map of the runs before this thread's, in its wave
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float pa = __shfl_up(A[j], kLanes), pb = __shfl_up(B[j], kLanes);
+    A[j] = lane < kLanes ? 1.f : pa;
+    B[j] = lane < kLanes ? 0.f : pb;
+  }
+  __syncthreads();
+
+  // the state before the piece
+  const int c = threadIdx.x % CW, p = threadIdx.x / CW, member = static_cast<int>(behind % P);
+  const bool mine = tile + c < a.width;
+  const float* start = BACK ? a.grad_final : a.state;
+  float ma = 1.f, mb = 0.f;                                               // the piece's own map, in the threads with p == 0
+  if (p == 0 && mine) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      mb = __builtin_fmaf(maps[0][w][c], mb, maps[1][w][c]);
+      ma *= maps[0][w][c];
+    }
+  }
+  const size_t group = static_cast<size_t>(column) * ((chunks + P - 1) / P) + behind / P;
+  if (W == 8 && chunks > 1) {
+    unsigned long long* words = board.maps + (static_cast<size_t>(column) * chunks + behind) * CW + c;
+    if (p == 0 && mine && behind < last && member < P - 1)
+      __hip_atomic_store(words, static_cast<unsigned long long>(word_of(ma)) << 32 | word_of(mb), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (mine && p < member) {
+      unsigned long long w;
+      while ((w = __hip_atomic_load(words - static_cast<int64_t>(member - p) * CW, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == ~0ull)
+        __builtin_amdgcn_s_sleep(1);
+      others[0][p][c] = __uint_as_float(static_cast<unsigned int>(w >> 32));
+      others[1][p][c] = __uint_as_float(static_cast<unsigned int>(w));
+    }
+  }
+  if (mine && p == P - 1) {
+    float h;
+    if (behind < P) {
+      h = start ? start[b * a.width + tile + c] : 0.f;
+    } else {
+      unsigned int w;
+      while ((w = __hip_atomic_load(board.states + (group - 1) * CW + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == kEmpty)
+        __builtin_amdgcn_s_sleep(1);
+      h = __uint_as_float(w);
+    }
+    before[c] = h;
+  }
+  __syncthreads();
+  if (p == 0 && mine) {
+    float h = before[c];
+    for (int i = 0; i < member; ++i) h = __builtin_fmaf(others[0][i][c], h, others[1][i][c]);
+    before[c] = h;
+    const float next = __builtin_fmaf(ma, h, mb);
+    if (behind == last) {
+      if (a.final_state) a.final_state[b * a.width + tile + c] = next;
+    } else if (member == P - 1) {
+      __hip_atomic_store(board.states + group * CW + c, word_of(next), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  __syncthreads();
+  if (nc <= 0) return;
+  float h[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) h[j] = before[(lane % kLanes) * N + j];
+  for (int w = 0; w < wave; ++w)
+#pragma unroll
+    for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(maps[0][w][(lane % kLanes) * N + j], h[j], maps[1][w][(lane % kLanes) * N + j]);
+#pragma unroll
+  for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(A[j], h[j], B[j]);
+
+  if constexpr (!BACK) {
+    const PieceRows<DT, FAR> out(a.out, b, k * RUN, tile);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      float g[N], x[N];
+      step_of<DT, LOG>(vg[i], vx[i], true, g, x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(g[j], h[j], x[j]);
+      if (row + i < rows) store_channels<DT>(out.at(row + i, cb), nc, h);
+    }
+  } else {
+    const PieceRows<DT, FAR> dg(a.grad_gate, b, k * RUN, tile), dx(a.grad_x, b, k * RUN, tile);
+    u32x4 vh[kSteps];
+    // h of the step before each: the rows from the piece before's last on; the first step of all has the state
+    const int first = k > 0 ? 1 : 0;
+    if (n > 0) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, vh);
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+      if (row + i >= rows) continue;                                       // h stays what came from behind
+      float g[N], x[N], prev[N];
+      step_of<DT, LOG>(vg[i], vx[i], true, g, x);
+      Elem<DT>::unpack(vh[i], prev);
+      if (i == 0 && row == 0 && k == 0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) prev[j] = a.state && j < nc ? a.state[b * a.width + c0 + j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        x[j] += h[j];                                                     // lambda
+        prev[j] *= x[j];
+        if (LOG) prev[j] *= g[j];
+        h[j] = g[j] * x[j];
+      }
+      store_channels<DT>(dx.at(row + i, cb), nc, x);
+      store_channels<DT>(dg.at(row + i, cb), nc, prev);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void clear_board(unsigned int* p, size_t n) {
+  for (size_t i = blockIdx.x * size_t{256} + threadIdx.x; i < n; i += size_t{256} * gridDim.x) p[i] = kEmpty;
 }
 
 template <class F> hipError_t by_type(int dtype, F&& f) {
@@ -58,24 +308,62 @@ template <class F> hipError_t by_type(int dtype, F&& f) {
   }
 }
 
+struct Plan {
+  int waves;
+  int64_t chunks, tiles, groups;
+};
+// Whether a piece's rows may lie further apart than 32-bit offsets reach.
+bool far_apart(const ScanArgs& a) {
+  int64_t step = 0;
+  for (int64_t s : {a.gate.step, a.x.step, a.out.step, a.grad_gate.step, a.grad_x.step}) step = step > s ? step : s;
+  return step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 + 1) >= (int64_t{1} << 32);
+}
+Plan plan_of(const ScanArgs& a) {
+  const int cw = kLanes * (16 / static_cast<int>(elem_size(a.dtype)));
+  const int waves = far_apart(a) ? 8 : a.time <= 64 ? 1 : a.time <= 256 ? 4 : 8;
+  const int64_t run = waves * 64;
+  const int64_t chunks = a.time > 0 ? (a.time + run - 1) / run : 1, per = 64 * waves / cw;
+  return {waves, chunks, (a.width + cw - 1) / cw, (chunks + per - 1) / per};
+}
+
+template <bool BACK> hipError_t launch(const ScanArgs& a, int compute_units, hipStream_t stream) {
+  const Plan p = plan_of(a);
+  Board board{};
+  if (p.chunks > 1) {
+    const size_t words = scan_workspace(a, compute_units) / 4;
+    board.ticket = static_cast<unsigned int*>(a.workspace);
+    board.maps = reinterpret_cast<unsigned long long*>(board.ticket + kTicketBytes / 4);
+    board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.chunks * kLanes * (16 / static_cast<int64_t>(elem_size(a.dtype))));
+    const size_t blocks = (words + 1023) / 1024;
+    clear_board<<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), 256, 0, stream>>>(board.ticket, words);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  const dim3 grid(static_cast<unsigned>(a.batch * p.tiles * p.chunks));
+  return by_type(a.dtype, [&](auto dt) {
+    auto go = [&](auto waves, auto is_far, auto eu) {
+      const int chunks = static_cast<int>(p.chunks), tiles = static_cast<int>(p.tiles);
+      if (a.log_gate) scan_chunks<dt.value, waves.value, BACK, true, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, chunks, tiles, board);
+      else scan_chunks<dt.value, waves.value, BACK, false, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, chunks, tiles, board);
+      return hipGetLastError();
+    };
+    const std::integral_constant<int, 2> two;
+    if (far_apart(a)) return go(std::integral_constant<int, 8>{}, std::true_type{}, two);
+    if (p.waves == 1) return go(std::integral_constant<int, 1>{}, std::false_type{}, two);
+    if (p.waves == 4) return go(std::integral_constant<int, 4>{}, std::false_type{}, two);
+    return go(std::integral_constant<int, 8>{}, std::false_type{}, std::integral_constant<int, 4>{});
+  });
+}
+
 }  // namespace
 
-size_t scan_workspace(const ScanArgs&, int) { return 0; }
-
-hipError_t launch_scan(const ScanArgs& a, int, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.batch * ((a.width + 63) / 64)));
-  return by_type(a.dtype, [&](auto dt) {
-    scan_steps<dt.value><<<grid, 64, 0, stream>>>(a);
-    return hipGetLastError();
-  });
+size_t scan_workspace(const ScanArgs& a, int) {
+  const Plan p = plan_of(a);
+  if (p.chunks <= 1) return 0;
+  const size_t cw = kLanes * (16 / elem_size(a.dtype));
+  return kTicketBytes + static_cast<size_t>(a.batch * p.tiles) * cw * (8 * static_cast<size_t>(p.chunks) + 4 * static_cast<size_t>(p.groups));
 }
 
-hipError_t launch_scan_grad(const ScanArgs& a, int, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.batch * ((a.width + 63) / 64)));
-  return by_type(a.dtype, [&](auto dt) {
-    scan_grad_steps<dt.value><<<grid, 64, 0, stream>>>(a);
-    return hipGetLastError();
-  });
-}
+hipError_t launch_scan(const ScanArgs& a, int compute_units, hipStream_t stream) { return launch<false>(a, compute_units, stream); }
+hipError_t launch_scan_grad(const ScanArgs& a, int compute_units, hipStream_t stream) { return launch<true>(a, compute_units, stream); }
 
 }  // namespace eh
