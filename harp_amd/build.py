@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libeclat_hip.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
-SOURCES = ["ast.cpp", "analysis.cpp", "normalize.cpp", "codegen.cpp", "stages.cpp", "rewrites.cpp", "plan.cpp", "emitters.cpp", "launches.cpp", "gemm.cpp", "window.cpp", "backend.cpp", "capi.cpp", "operators.cpp"]
+SOURCES = ["ast.cpp", "analysis.cpp", "normalize.cpp", "codegen.cpp", "stages.cpp", "rewrites.cpp", "plan.cpp", "emitters.cpp", "launches.cpp", "gemm.cpp", "window.cpp", "backend.cpp", "capi.cpp", "operators.cpp", "operator_plans.cpp"]
 # compiled as HIP for gfx950: the library's one statically allocated device array and the kernels that
 # are compiled ahead of time
 DEVICE_SOURCES = ["static_scratch.hip", "kernels/token_rows.hip", "kernels/gated_scan.hip"]

@@ -20,6 +20,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 template <int DT> struct Elem;
 
 template <> struct Elem<kF32> {
+  static constexpr uint32_t kMinusInfinity = 0xff800000u;       // a word of them
   static constexpr int N = 4;                              // elements in 16 bytes
   typedef float T;
   __device__ static void unpack(u32x4 v, float* z) {
@@ -37,6 +38,7 @@ template <> struct Elem<kF32> {
 };
 
 template <> struct Elem<kBF16> {
+  static constexpr uint32_t kMinusInfinity = 0xff80ff80u;       // a word of them
   static constexpr int N = 8;
   typedef uint16_t T;
   __device__ static void unpack(u32x4 v, float* z) {
@@ -60,6 +62,7 @@ template <> struct Elem<kBF16> {
 };
 
 template <> struct Elem<kF16> {
+  static constexpr uint32_t kMinusInfinity = 0xfc00fc00u;       // a word of them
   static constexpr int N = 8;
   typedef uint16_t T;
   __device__ static void unpack(u32x4 v, float* z) {
@@ -85,6 +88,8 @@ template <> struct Elem<kF16> {
 
 __device__ inline u32x4 load16(const void* p) { return *static_cast<const u32x4_any*>(p); }
 __device__ inline void store16(void* p, u32x4 v) { *static_cast<u32x4_any*>(p) = v; }
+// (past the caches: for results that a launch larger than they are does not read again)
+__device__ inline void stream16(void* p, u32x4 v) { __builtin_nontemporal_store(v, static_cast<u32x4_any*>(p)); }
 
 // An element of a run-time type: for the few values a row has besides its logits.
 __device__ inline float load_as(const void* p, int64_t i, int dtype) {
@@ -152,6 +157,21 @@ template <int THREADS> __device__ inline float block_sum(float x, float* lds) {
   for (int i = 1; i < THREADS / 64; ++i) s += lds[i];
   __syncthreads();
   return s;
+}
+// Two sums at once; `lds` holds two values per wave.
+template <int THREADS> __device__ inline void block_sum(float& x, float& y, float* lds) {
+  x = wave_sum(x);
+  y = wave_sum(y);
+  if constexpr (THREADS == 64) {
+    __syncthreads();                      // what lanes have left in LDS is there for the others here too
+    return;
+  }
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x, lds[THREADS / 64 + (threadIdx.x >> 6)] = y;
+  __syncthreads();
+  x = lds[0], y = lds[THREADS / 64];
+#pragma unroll
+  for (int i = 1; i < THREADS / 64; ++i) x += lds[i], y += lds[THREADS / 64 + i];
+  __syncthreads();
 }
 template <int THREADS> __device__ inline float block_max(float x, float* lds) {
   x = wave_max(x);

@@ -9,8 +9,8 @@
 namespace eh {
 namespace {
 
-constexpr int kSteps = 8;            // a thread's own steps, held in registers from the only reading
-constexpr int kLanes = 8;            // lanes side by side: 128 bytes of a step, a whole cache line
+constexpr int kSteps = kScanSteps;   // a thread's own steps, held in registers from the only reading
+constexpr int kLanes = kScanLanes;   // lanes side by side: 128 bytes of a step, a whole cache line
 
 template <int DT> struct Chunk {
   static constexpr int N = Elem<DT>::N;
@@ -26,7 +26,6 @@ struct Board {
   unsigned int* states;
 };
 constexpr unsigned int kEmpty = 0xffffffffu;
-constexpr size_t kTicketBytes = 256;
 
 __device__ inline unsigned int word_of(float x) {
   const unsigned int b = __float_as_uint(x);
@@ -308,46 +307,28 @@ template <class F> hipError_t by_type(int dtype, F&& f) {
   }
 }
 
-struct Plan {
-  int waves;
-  int64_t chunks, tiles, groups;
-};
-// Whether a piece's rows may lie further apart than 32-bit offsets reach.
-bool far_apart(const ScanArgs& a) {
-  int64_t step = 0;
-  for (int64_t s : {a.gate.step, a.x.step, a.out.step, a.grad_gate.step, a.grad_x.step}) step = step > s ? step : s;
-  return step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 + 1) >= (int64_t{1} << 32);
-}
-Plan plan_of(const ScanArgs& a) {
-  const int cw = kLanes * (16 / static_cast<int>(elem_size(a.dtype)));
-  const int waves = far_apart(a) ? 8 : a.time <= 64 ? 1 : a.time <= 256 ? 4 : 8;
-  const int64_t run = waves * 64;
-  const int64_t chunks = a.time > 0 ? (a.time + run - 1) / run : 1, per = 64 * waves / cw;
-  return {waves, chunks, (a.width + cw - 1) / cw, (chunks + per - 1) / per};
-}
-
-template <bool BACK> hipError_t launch(const ScanArgs& a, int compute_units, hipStream_t stream) {
-  const Plan p = plan_of(a);
+template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
+  const ScanPlan p = plan_scan(a);
   Board board{};
-  if (p.chunks > 1) {
-    const size_t words = scan_workspace(a, compute_units) / 4;
+  if (p.pieces > 1) {
+    const size_t words = scan_workspace(a) / 4;
     board.ticket = static_cast<unsigned int*>(a.workspace);
     board.maps = reinterpret_cast<unsigned long long*>(board.ticket + kTicketBytes / 4);
-    board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.chunks * kLanes * (16 / static_cast<int64_t>(elem_size(a.dtype))));
+    board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.pieces * p.channels);
     const size_t blocks = (words + 1023) / 1024;
     clear_board<<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), 256, 0, stream>>>(board.ticket, words);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  const dim3 grid(static_cast<unsigned>(a.batch * p.tiles * p.chunks));
+  const dim3 grid(static_cast<unsigned>(a.batch * p.tiles * p.pieces));
   return by_type(a.dtype, [&](auto dt) {
     auto go = [&](auto waves, auto is_far, auto eu) {
-      const int chunks = static_cast<int>(p.chunks), tiles = static_cast<int>(p.tiles);
-      if (a.log_gate) scan_chunks<dt.value, waves.value, BACK, true, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, chunks, tiles, board);
-      else scan_chunks<dt.value, waves.value, BACK, false, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, chunks, tiles, board);
+      const int pieces = static_cast<int>(p.pieces), tiles = static_cast<int>(p.tiles);
+      if (a.log_gate) scan_chunks<dt.value, waves.value, BACK, true, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, board);
+      else scan_chunks<dt.value, waves.value, BACK, false, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, board);
       return hipGetLastError();
     };
     const std::integral_constant<int, 2> two;
-    if (far_apart(a)) return go(std::integral_constant<int, 8>{}, std::true_type{}, two);
+    if (p.far) return go(std::integral_constant<int, 8>{}, std::true_type{}, two);
     if (p.waves == 1) return go(std::integral_constant<int, 1>{}, std::false_type{}, two);
     if (p.waves == 4) return go(std::integral_constant<int, 4>{}, std::false_type{}, two);
     return go(std::integral_constant<int, 8>{}, std::false_type{}, std::integral_constant<int, 4>{});
@@ -356,14 +337,7 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, int compute_units, hip
 
 }  // namespace
 
-size_t scan_workspace(const ScanArgs& a, int) {
-  const Plan p = plan_of(a);
-  if (p.chunks <= 1) return 0;
-  const size_t cw = kLanes * (16 / elem_size(a.dtype));
-  return kTicketBytes + static_cast<size_t>(a.batch * p.tiles) * cw * (8 * static_cast<size_t>(p.chunks) + 4 * static_cast<size_t>(p.groups));
-}
-
-hipError_t launch_scan(const ScanArgs& a, int compute_units, hipStream_t stream) { return launch<false>(a, compute_units, stream); }
-hipError_t launch_scan_grad(const ScanArgs& a, int compute_units, hipStream_t stream) { return launch<true>(a, compute_units, stream); }
+hipError_t launch_scan(const ScanArgs& a, hipStream_t stream) { return launch<false>(a, stream); }
+hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t stream) { return launch<true>(a, stream); }
 
 }  // namespace eh

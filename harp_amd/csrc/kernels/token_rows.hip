@@ -14,18 +14,32 @@ namespace {
 constexpr float kLowest = -3.402823466e+38f;
 constexpr int kCandidates = 512;          // elements at or above the selection's threshold that LDS holds
 
-__device__ inline int row_vectors(int n, int per) { return (n + per - 1) / per; }
-
-// Elements [N * i, N * i + N) of a row's segment of n elements; those at n and behind are -infinity.
-template <int DT> __device__ inline void load_vector(const typename Elem<DT>::T* p, int i, int n, float* z) {
-  constexpr int N = Elem<DT>::N;
-  if ((i + 1) * N <= n) {
-    Elem<DT>::unpack(load16(p + static_cast<int64_t>(i) * N), z);
-  } else {
+// A segment of a row as items of N elements that start at 16-byte boundaries, whatever the row's own
+// start: item i has elements [N i - skew, N i - skew + N) of the segment, the first and the last item
+// perhaps fewer.  (Vectors from an odd address cost a sixth of a reading pass's rate in 16-bit types.)
+template <int DT> struct Segment {
+  static constexpr int N = Elem<DT>::N;
+  typedef typename Elem<DT>::T T;
+  const T* p;
+  int n, skew;
+  __device__ Segment(const T* p_, int n_) : p(p_), n(n_), skew(static_cast<int>(reinterpret_cast<uintptr_t>(p_) / sizeof(T) % N)) {}
+  __device__ int items() const { return (n + skew + N - 1) / N; }
+  __device__ int full() const { return (n + skew) / N; }              // items before this one reach to their end
+  __device__ int place(int i, int j) const { return i * N + j - skew; }
+  __device__ u32x4 vector(int i) const { return *reinterpret_cast<const u32x4*>(p + (static_cast<int64_t>(i) * N - skew)); }
+  // any item; what is not of the segment is -infinity
+  __device__ void load(int i, float* z) const {
+    if (i * N >= skew && i < full()) {
+      Elem<DT>::unpack(vector(i), z);
+    } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = i * N + j < n ? Elem<DT>::get(p[i * N + j]) : -INFINITY;
+      for (int j = 0; j < N; ++j) {
+        const int at = place(i, j);
+        z[j] = at >= 0 && at < n ? Elem<DT>::get(p[at]) : -INFINITY;
+      }
+    }
   }
-}
+};
 
 // ---- one pass over a row: running maximum, sum of exponentials, sum of their arguments -------------
 
@@ -58,23 +72,29 @@ template <int COUNT, bool ENT> __device__ inline void add_elements(RowSums& a, c
   }
 }
 
-template <int DT, int THREADS, bool ENT> __device__ inline RowSums sum_row(const typename Elem<DT>::T* p, int n, float c2) {
+template <int DT, int THREADS, bool ENT> __device__ inline RowSums sum_row(const Segment<DT>& row, float c2) {
   constexpr int N = Elem<DT>::N, U = 4;
-  const int full = n / N, all = row_vectors(n, N);
+  const int full = row.full(), items = row.items();
   RowSums a;
   int i = threadIdx.x;
+  if (row.skew && i == 0) {
+    float z[N];
+    row.load(0, z);
+    add_elements<N, ENT>(a, z, c2);
+    i += THREADS;
+  }
   for (; i + (U - 1) * THREADS < full; i += U * THREADS) {
     u32x4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load16(p + static_cast<int64_t>(i + u * THREADS) * N);
+    for (int u = 0; u < U; ++u) v[u] = row.vector(i + u * THREADS);
     float z[U * N];
 #pragma unroll
     for (int u = 0; u < U; ++u) Elem<DT>::unpack(v[u], z + u * N);
     add_elements<U * N, ENT>(a, z, c2);
   }
-  for (; i < all; i += THREADS) {
+  for (; i < items; i += THREADS) {
     float z[N];
-    load_vector<DT>(p, i, n, z);
+    row.load(i, z);
     add_elements<N, ENT>(a, z, c2);
   }
   return a;
@@ -107,47 +127,86 @@ __device__ inline uint32_t place_of(uint64_t key) { return 0xffffffffu - static_
 
 struct Selection {
   uint32_t group[64];
-  int count;
+  int count, owners;
+  uint16_t owner[1024];
   uint64_t found[kCandidates];
   uint64_t top[kMaxTop];
 };
 
-// A segment of a row: thread t has vectors t, t + THREADS, ...  `base` is the segment's place in its row.
-template <int DT, int THREADS> struct RowSource {
+// What is selected from is spread over the threads: item i of the source is thread i % THREADS's.  A
+// source gives the (order, place) pairs of `U` items at a time, so that their loads overlap.
+
+// A segment of a row by its items; `base` is the segment's place in its row.
+template <int DT> struct RowSource {
+  static constexpr int N = Elem<DT>::N, U = 4;
+  Segment<DT> row;
+  int base;
+  __device__ int items() const { return row.items(); }
+  template <class F> __device__ void visit(const int* item, F&& f) const {
+    float z[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (item[u] >= 0) row.load(item[u], z[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (item[u] < 0) continue;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int at = row.place(item[u], j);
+        if (const uint32_t order = order_of(z[u][j]); order && at >= 0 && at < row.n) f(order, static_cast<uint32_t>(base + at));
+      }
+    }
+  }
+};
+// The same with an item an element: rows too short to give every thread a vector.
+template <int DT> struct ElementSource {
+  static constexpr int U = 4;
   const typename Elem<DT>::T* p;
   int n, base;
-  template <class F> __device__ void each(F&& f) const {
-    constexpr int N = Elem<DT>::N;
-    const int all = row_vectors(n, N);
-    for (int i = threadIdx.x; i < all; i += THREADS) {
-      float z[N];
-      load_vector<DT>(p, i, n, z);
+  __device__ int items() const { return n; }
+  template <class F> __device__ void visit(const int* item, F&& f) const {
+    float z[U];
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (const uint32_t order = order_of(z[j]); order && i * N + j < n) f(order, static_cast<uint32_t>(base + i * N + j));
-    }
+    for (int u = 0; u < U; ++u) z[u] = item[u] >= 0 ? Elem<DT>::get(p[item[u]]) : __builtin_nanf("");
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (const uint32_t order = order_of(z[u])) f(order, static_cast<uint32_t>(base + item[u]));
   }
 };
 // Keys in memory (0: none).
-template <int THREADS> struct KeySource {
+struct KeySource {
+  static constexpr int U = 4;
   const uint64_t* keys;
   int n;
-  template <class F> __device__ void each(F&& f) const {
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      const uint64_t k = keys[i];
-      if (k) f(static_cast<uint32_t>(k >> 32), place_of(k));
-    }
+  __device__ int items() const { return n; }
+  template <class F> __device__ void visit(const int* item, F&& f) const {
+    uint64_t k[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) k[u] = item[u] >= 0 ? keys[item[u]] : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k[u]) f(static_cast<uint32_t>(k[u] >> 32), place_of(k[u]));
   }
 };
+template <int THREADS, class Source, class F> __device__ inline void visit_own(const Source& src, F&& f) {
+  const int items = src.items();
+  for (int i = threadIdx.x; i < items; i += Source::U * THREADS) {
+    int item[Source::U];
+#pragma unroll
+    for (int u = 0; u < Source::U; ++u) item[u] = i + u * THREADS < items ? i + u * THREADS : -1;
+    src.visit(item, f);
+  }
+}
 
 // Leaves the k largest keys of `src` in sel.top, largest first (0 behind the last where there are
 // fewer).  `mine`: the largest order among the thread's own elements, 0 if it has none.
 //
 // The threads form 64 groups.  The k-th largest of the groups' maxima is no larger than the row's
 // k-th largest element, so the k are among the elements at or above it, about as many as k in a
-// row without structure: only threads that have one read theirs again.  A wave finds that
-// threshold bit by bit with ballots.  A row with many elements there (equal ones, say) takes k
-// rounds over the row instead.
+// row without structure: only the items of threads that have one are read again, by all threads
+// together (by the thread itself that was 25 us of latency for a row of 50000, 3.4 us a row with
+// eight rows on a compute unit).  A wave finds the threshold bit by bit with ballots.  A row with
+// many elements there (equal ones, say) takes k rounds over the row instead.
 template <int THREADS, class Source>
 __device__ inline void select_top(const Source& src, uint32_t mine, int k, Selection& sel) {
   constexpr int G = THREADS / 64;
@@ -157,7 +216,7 @@ __device__ inline void select_top(const Source& src, uint32_t mine, int k, Selec
   if (G >= 8) g = max(g, dpp<kHalfMirror>(g, g));
   if (G >= 16) g = max(g, dpp<kMirror>(g, g));
   if (threadIdx.x % G == 0) sel.group[threadIdx.x / G] = g;
-  if (threadIdx.x == 0) sel.count = 0;
+  if (threadIdx.x == 0) sel.count = sel.owners = 0;
   if (threadIdx.x < kMaxTop) sel.top[threadIdx.x] = 0;
   __syncthreads();
   g = sel.group[threadIdx.x & 63];
@@ -165,66 +224,84 @@ __device__ inline void select_top(const Source& src, uint32_t mine, int k, Selec
 #pragma unroll 1
   for (int b = 31; b >= 0; --b) {
     const uint32_t t = tau | 1u << b;
-    if (static_cast<int>(__popcll(__ballot(g >= t))) >= k) tau = t;
+    const int above = static_cast<int>(__popcll(__ballot(g >= t)));
+    if (above >= k) tau = t;
+    if (above == k) break;                                  // lower bits would not part the groups any more
   }
-  if (mine && mine >= tau)
-    src.each([&](uint32_t order, uint32_t place) {
+  if (mine && mine >= tau) sel.owner[atomicAdd(&sel.owners, 1)] = static_cast<uint16_t>(threadIdx.x);
+  __syncthreads();
+  const int owners = sel.owners, items = src.items(), total = owners * ((items + THREADS - 1) / THREADS);
+  for (int i = threadIdx.x; i < total; i += Source::U * THREADS) {
+    int item[Source::U];
+#pragma unroll
+    for (int u = 0; u < Source::U; ++u) {
+      const int at = i + u * THREADS;
+      item[u] = at < total ? sel.owner[at % owners] + at / owners * THREADS : -1;
+      if (item[u] >= items) item[u] = -1;
+    }
+    src.visit(item, [&](uint32_t order, uint32_t place) {
       if (order >= tau) {
-        const int at = atomicAdd(&sel.count, 1);
-        if (at < kCandidates) sel.found[at] = key_of(order, place);
+        const int found = atomicAdd(&sel.count, 1);
+        if (found < kCandidates) sel.found[found] = key_of(order, place);
       }
     });
+  }
   __syncthreads();
   const int count = sel.count;
   if (count <= kCandidates) {
     for (int i = threadIdx.x; i < count; i += THREADS) {
       const uint64_t key = sel.found[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < count; ++j) rank += sel.found[j] > key;
       if (rank < k) sel.top[rank] = key;
     }
   } else {
-    uint64_t last = ~uint64_t{0};
-    uint64_t* best = sel.found;
+    unsigned long long last = ~0ull;
     for (int r = 0; r < k; ++r) {
-      uint64_t b = 0;
-      src.each([&](uint32_t order, uint32_t place) {
+      unsigned long long b = 0;
+      visit_own<THREADS>(src, [&](uint32_t order, uint32_t place) {
         const uint64_t key = key_of(order, place);
         if (key < last && key > b) b = key;
       });
+      for (int off = 32; off > 0; off /= 2) b = max(b, __shfl_xor(b, off));
+      __syncthreads();                                      // everybody has read the round before's
+      if ((threadIdx.x & 63) == 0) sel.found[threadIdx.x / 64] = b;
       __syncthreads();
-      best[threadIdx.x] = b;
-      __syncthreads();
-      for (int h = THREADS / 2; h > 0; h >>= 1) {
-        if (static_cast<int>(threadIdx.x) < h && best[threadIdx.x + h] > best[threadIdx.x]) best[threadIdx.x] = best[threadIdx.x + h];
-        __syncthreads();
-      }
-      last = best[0];
+      last = sel.found[0];
+      for (int w = 1; w < THREADS / 64; ++w) last = max(last, static_cast<unsigned long long>(sel.found[w]));
       if (threadIdx.x == 0) sel.top[r] = last;
     }
   }
   __syncthreads();
 }
-static_assert(kCandidates >= 512, "the rounds over a row use a key per thread");
+static_assert(kCandidates >= 1024 / 64, "the rounds over a row use a key per wave");
 
 // ---- token log probabilities ---------------------------------------------------------------------------
 
-struct Partial {                 // a segment's sums; its best keys follow all rows' partials
-  float largest, s, t, pad;
+// (a segment's sums go to the workspace as a Partial; its best keys follow all rows' partials)
+typedef RowPartial Partial;
+
+// The given token's logit; read ahead of the sums, so that nobody waits for it behind them.
+struct Target {
+  int64_t id;
+  float z;
+  __device__ Target(const ScoreArgs& a, int64_t row) : id(load_id(a.targets, row)), z(0.f) {
+    if (id >= 0 && id < a.in.vocab) z = load_as(a.in.z, row * a.in.stride + id, a.in.dtype);
+  }
 };
 
 // What a row reports, once its sums (and best keys) are known.  All threads of the workgroup call it.
-__device__ inline void report_row(const ScoreArgs& a, int64_t row, const RowSums& r, const Selection* sel) {
+__device__ inline void report_row(const ScoreArgs& a, int64_t row, const RowSums& r, const Target& target, const Selection* sel) {
   const float scale = a.in.scale;
   const bool empty = r.s == 0.f;                            // no element above -infinity
   const float log_s = log2_hw(r.s) * kLn2;
   if (threadIdx.x == 0) {
-    const int64_t id = load_id(a.targets, row);
+    const int64_t id = target.id;
     float lp = 0.f;
     if (id != a.ignore) {
       lp = __builtin_nanf("");
-      if (id >= 0 && id < a.in.vocab)
-        lp = empty ? -INFINITY : (load_as(a.in.z, row * a.in.stride + id, a.in.dtype) - r.m) * scale - log_s;
+      if (id >= 0 && id < a.in.vocab) lp = empty ? -INFINITY : (target.z - r.m) * scale - log_s;
     }
     a.logp[row] = lp;
     a.norm[2 * row] = r.largest;
@@ -249,15 +326,23 @@ template <int DT, int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(
   const int n = min(a.split.seg, a.in.vocab - lo);
   const auto* p = static_cast<const typename Elem<DT>::T*>(a.in.z) + row * a.in.stride + lo;
   const float c2 = a.in.scale * kLog2e;
-  const RowSums mine = sum_row<DT, THREADS, ENT>(p, n, c2);
+  const Target target(a, row);
+  const Segment<DT> part(p, n);
+  const RowSums mine = sum_row<DT, THREADS, ENT>(part, c2);
   const RowSums r = join_row<THREADS, ENT>(mine, c2, lds);
   if constexpr (TOP) {
-    const bool has = static_cast<int>(threadIdx.x) < row_vectors(n, Elem<DT>::N);
-    select_top<THREADS>(RowSource<DT, THREADS>{p, n, lo}, has ? order_of(mine.largest) : 0u, a.top, sel);
+    if (part.items() >= THREADS) {
+      select_top<THREADS>(RowSource<DT>{part, lo}, order_of(mine.largest), a.top, sel);
+    } else {
+      const ElementSource<DT> src{p, n, lo};
+      uint32_t largest = 0;
+      visit_own<THREADS>(src, [&](uint32_t order, uint32_t) { largest = max(largest, order); });
+      select_top<THREADS>(src, largest, a.top, sel);
+    }
   }
   if (a.split.segs == 1) {
-    if constexpr (TOP) report_row(a, row, r, &sel);
-    else report_row(a, row, r, nullptr);
+    if constexpr (TOP) report_row(a, row, r, target, &sel);
+    else report_row(a, row, r, target, nullptr);
     return;
   }
   Partial* parts = static_cast<Partial*>(a.workspace);
@@ -268,8 +353,8 @@ template <int DT, int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(
   }
 }
 
-// The sums of a row's segments as the row's, in every thread.
-template <int THREADS, bool ENT> __device__ inline RowSums join_parts(const Partial* parts, int segs, float c2, float* lds) {
+// This thread's share of the sums of a row's segments.
+template <int THREADS, bool ENT> __device__ inline RowSums add_parts(const Partial* parts, int segs, float c2) {
   RowSums a;
   for (int i = threadIdx.x; i < segs; i += THREADS) {
     const Partial p = parts[i];
@@ -282,7 +367,7 @@ template <int THREADS, bool ENT> __device__ inline RowSums join_parts(const Part
     a.s += b.s;
     a.t += b.t;
   }
-  return join_row<THREADS, ENT>(a, c2, lds);
+  return a;
 }
 
 template <int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS) void score_join(ScoreArgs a) {
@@ -291,28 +376,38 @@ template <int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS)
   const int64_t row = blockIdx.x;
   const int segs = a.split.segs;
   const Partial* parts = static_cast<const Partial*>(a.workspace);
-  const RowSums r = join_parts<THREADS, ENT>(parts + row * segs, segs, a.in.scale * kLog2e, lds);
+  const Target target(a, row);
+  const RowSums r = join_row<THREADS, ENT>(add_parts<THREADS, ENT>(parts + row * segs, segs, a.in.scale * kLog2e), a.in.scale * kLog2e, lds);
   if constexpr (TOP) {
     const uint64_t* keys = reinterpret_cast<const uint64_t*>(parts + a.in.rows * segs) + row * segs * a.top;
-    const KeySource<THREADS> src{keys, segs * a.top};
+    const KeySource src{keys, segs * a.top};
     uint32_t mine = 0;
-    src.each([&](uint32_t order, uint32_t) { mine = max(mine, order); });
+    visit_own<THREADS>(src, [&](uint32_t order, uint32_t) { mine = max(mine, order); });
     select_top<THREADS>(src, mine, a.top, sel);
-    report_row(a, row, r, &sel);
+    report_row(a, row, r, target, &sel);
   } else {
-    report_row(a, row, r, nullptr);
+    report_row(a, row, r, target, nullptr);
   }
 }
 
 // dz_i = c [ g ([i = t] - p_i) - e p_i (log p_i + H) ] with g, e the gradients of log p_t and H: one
-// pass, a workgroup for `span` elements of a row.
-template <int DT, bool ENT> __global__ __launch_bounds__(256) void score_grad_rows(ScoreGradArgs a, int spans, int span) {
-  constexpr int N = Elem<DT>::N, U = 4, THREADS = 256;
+// pass, a vector for each thread.  Workgroups of 4 KB keep what is on the way in memory order:
+// 8192 x 65536 bf16 in 337 us (6.4 TB/s); 362 us with two vectors a thread, 415 us with a row for a workgroup.
+template <int DT, bool ENT> __global__ __launch_bounds__(256) void score_grad_rows(ScoreGradArgs a, int spans) {
+  constexpr int N = Elem<DT>::N;
   typedef typename Elem<DT>::T T;
   const int64_t row = blockIdx.x / spans;
-  const int lo = static_cast<int>(blockIdx.x % spans) * span, n = min(span, a.in.vocab - lo);
-  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride + lo;
-  T* out = static_cast<T*>(a.grad) + row * a.grad_stride + lo;
+  const int at = (static_cast<int>(blockIdx.x % spans) * 256 + static_cast<int>(threadIdx.x)) * N, n = a.in.vocab - at;
+  if (n <= 0) return;
+  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride + at;
+  T* out = static_cast<T*>(a.grad) + row * a.grad_stride + at;
+  float z[N];
+  if (n >= N) {
+    Elem<DT>::unpack(load16(p), z);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = j < n ? Elem<DT>::get(p[j]) : 0.f;
+  }
   const float m = a.norm[2 * row], log_s = a.norm[2 * row + 1], scale = a.in.scale;
   const bool empty = m == -INFINITY && log_s == -INFINITY;
   const int64_t id = load_id(a.targets, row);
@@ -320,204 +415,305 @@ template <int DT, bool ENT> __global__ __launch_bounds__(256) void score_grad_ro
   const float e = ENT ? a.grad_entropy[row] : 0.f;
   if (id == a.ignore) g = 0.f;
   else if (id < 0 || id >= a.in.vocab) g = __builtin_nanf("");
-  const float at = scale * g, all = scale * (ENT ? g + e * a.entropy[row] : g), each = scale * e;
-  const int64_t target = id - lo;
-  auto gradient = [&](float z) {
-    const float lp = (z - m) * scale - log_s, pr = exp2_hw(lp * kLog2e);
-    return ENT ? -pr * (all + each * fmaxf(lp, -200.f)) : -pr * all;
-  };
-  auto vector = [&](int i, float* z) {
+  const float all = scale * (ENT ? g + e * a.entropy[row] : g), each = scale * e;
+  const int64_t target = id == a.ignore || empty ? -1 : id - at;
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = empty ? 0.f : gradient(z[j]);
-    const int64_t d = target - static_cast<int64_t>(i) * N;
-    if (d >= 0 && d < N && !empty && id != a.ignore) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) z[j] += j == d ? at : 0.f;
-    }
-  };
-  const int full = n / N, all_vectors = row_vectors(n, N);
-  int i = threadIdx.x;
-  for (; i + (U - 1) * THREADS < full; i += U * THREADS) {
-    u32x4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load16(p + static_cast<int64_t>(i + u * THREADS) * N);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float z[N];
-      Elem<DT>::unpack(v[u], z);
-      vector(i + u * THREADS, z);
-      store16(out + static_cast<int64_t>(i + u * THREADS) * N, Elem<DT>::pack(z));
-    }
+  for (int j = 0; j < N; ++j) {
+    const float lp = (z[j] - m) * scale - log_s, pr = exp2_hw(lp * kLog2e);
+    z[j] = empty ? 0.f : ENT ? -pr * (all + each * fmaxf(lp, -200.f)) : -pr * all;
+    if (j == target) z[j] += scale * g;
   }
-  for (; i < all_vectors; i += THREADS) {
-    float z[N];
-    load_vector<DT>(p, i, n, z);
-    vector(i, z);
-    if (i < full) {
-      store16(out + static_cast<int64_t>(i) * N, Elem<DT>::pack(z));
-    } else {
+  if (n >= N) {
+    stream16(out, Elem<DT>::pack(z));
+  } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (i * N + j < n) out[i * N + j] = Elem<DT>::put(z[j]);
-    }
+    for (int j = 0; j < N; ++j)
+      if (j < n) out[j] = Elem<DT>::put(z[j]);
   }
 }
 
 // ---- distillation --------------------------------------------------------------------------------------
 
+// The teacher's entries of a row, in as much LDS as they need, and for each thread the chain of those
+// whose elements it writes.
 struct Teacher {
-  int ids[kMaxTeacher];          // -1: no entry
-  float q[kMaxTeacher];
+  int* ids;                      // -1: no entry
+  int* next;                     // the next entry of the same owner, -1 behind the last
+  float* q;
+  float* log_q;
+  float* sum;                    // q of all entries that name the same token: one named twice counts twice
+  float* z;                      // the student's logit
+  int* head;                     // a thread's first entry, -1: none
+  __device__ Teacher(float* lds, int k)
+      : ids(reinterpret_cast<int*>(lds)), next(ids + k), q(lds + 2 * k), log_q(lds + 3 * k), sum(lds + 4 * k), z(lds + 5 * k),
+        head(ids + 6 * k) {}
+  static size_t bytes(int k, int threads) { return 24 * static_cast<size_t>(k) + 4 * static_cast<size_t>(threads); }
+};
+extern __shared__ float teacher_lds[];
+
+// A thread's first entry while it is on its way from memory.
+struct Entry {
+  int id;
+  float u;
+  __device__ Entry(const DistillArgs& a, int64_t row, int k) : id(-1), u(-INFINITY) {
+    if (k >= a.k) return;
+    const int64_t i = load_id(a.ids, row * a.ids_stride + k);
+    u = load_as(a.teacher, row * a.teacher_stride + k, a.teacher_dtype);
+    if (i >= 0 && i < a.in.vocab) id = static_cast<int>(i);
+  }
 };
 
-// The teacher's probabilities of a row into LDS (entries whose id is not a token have none); returns
-// sum q (1, or 0 where no entry has any) and, where `largest` is given, the row's loss / T^2:
-// sum_k q_k (log q_k - log p_(id_k)).
-template <int THREADS> __device__ inline float load_teacher(const DistillArgs& a, int64_t row, Teacher& t, float* lds,
-                                                            const RowSums* r, float* kl) {
+// The teacher's probabilities of a row into LDS: sum q is 1, or 0 where no entry has any, and is
+// returned.  Entries whose id is not a token have none.  OWNERS: the chains too; element i is written
+// by the thread that has vector i / N, behind the last whole vector by thread i - N * full.
+template <int THREADS, int N, bool OWNERS>
+__device__ inline float load_teacher(const DistillArgs& a, int64_t row, const Entry& first, const Teacher& t, float* lds) {
   const float inv = 1.f / a.temperature;
+  if (OWNERS) t.head[threadIdx.x] = -1;
   float m = -INFINITY;
   for (int k = threadIdx.x; k < a.k; k += THREADS) {
-    const int64_t id = load_id(a.ids, row * a.ids_stride + k);
-    const bool named = id >= 0 && id < a.in.vocab;
-    const float u = named ? load_as(a.teacher, row * a.teacher_stride + k, a.teacher_dtype) : -INFINITY;
-    t.ids[k] = named ? static_cast<int>(id) : -1;
+    const Entry e = k < THREADS ? first : Entry(a, row, k);
+    const float u = e.id >= 0 ? e.u : -INFINITY;
+    t.ids[k] = e.id;
     t.q[k] = u;
     m = u != u ? u : fmaxf(m, u);
   }
-  m = block_max<THREADS>(m, lds);
-  const float ref = fmaxf(m, kLowest);
+  m = fmaxf(block_max<THREADS>(m, lds), kLowest);
   float s = 0.f;
   for (int k = threadIdx.x; k < a.k; k += THREADS)
-    if (t.ids[k] >= 0) s += exp2_hw((t.q[k] - ref) * inv * kLog2e);
+    if (t.ids[k] >= 0) s += exp2_hw((t.q[k] - m) * inv * kLog2e);
   s = block_sum<THREADS>(s, lds);
   const float log_s = log2_hw(s) * kLn2;
   const bool none = s == 0.f;
-  const bool empty = r && r->s == 0.f;
-  const float log_z = r ? log2_hw(r->s) * kLn2 : 0.f;
-  float loss = 0.f;
   for (int k = threadIdx.x; k < a.k; k += THREADS) {
-    const float log_q = (t.q[k] - ref) * inv - log_s, q = t.ids[k] >= 0 && !none ? exp2_hw(log_q * kLog2e) : 0.f;
-    if (kl && q != 0.f) {
-      const float z = load_as(a.in.z, row * a.in.stride + t.ids[k], a.in.dtype);
-      loss += q * (log_q - (empty ? -INFINITY : (z - r->m) * a.in.scale - log_z));
-    }
-    t.q[k] = q;
-  }
-  if (kl) *kl = block_sum<THREADS>(loss, lds);
-  __syncthreads();                        // the entries are there for every thread
-  return none ? 0.f : 1.f;
-}
-
-// dz_i = w T (Q p_i - sum_{k: id_k = i} q_k) over [lo, lo + n) of a row.  p_i = exp2(c2 (z_i - m) - shift).
-// The entries that the teacher names are written again behind the barrier, from the logits themselves.
-template <int DT, int THREADS>
-__device__ inline void write_gradient(const DistillArgs& a, int64_t row, int lo, int n, float m, float shift, bool empty,
-                                      float w, float total, const Teacher& t) {
-  constexpr int N = Elem<DT>::N, U = 4;
-  typedef typename Elem<DT>::T T;
-  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride + lo;
-  T* out = static_cast<T*>(a.grad) + row * a.grad_stride + lo;
-  const float c2 = a.in.scale * kLog2e, coef = empty ? 0.f : w * total;
-  const float ref = empty ? INFINITY : m;             // every exponential of an empty row is 0
-  if (empty) shift = 0.f;
-  auto gradient = [&](float z) { return coef * exp2_hw(__builtin_fmaf(z - ref, c2, -shift)); };
-  const int full = n / N, all = row_vectors(n, N);
-  int i = threadIdx.x;
-  for (; i + (U - 1) * THREADS < full; i += U * THREADS) {
-    u32x4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load16(p + static_cast<int64_t>(i + u * THREADS) * N);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float z[N];
-      Elem<DT>::unpack(v[u], z);
-#pragma unroll
-      for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
-      store16(out + static_cast<int64_t>(i + u * THREADS) * N, Elem<DT>::pack(z));
-    }
-  }
-  for (; i < all; i += THREADS) {
-    float z[N];
-    load_vector<DT>(p, i, n, z);
-#pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
-    if (i < full) {
-      store16(out + static_cast<int64_t>(i) * N, Elem<DT>::pack(z));
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (i * N + j < n) out[i * N + j] = Elem<DT>::put(z[j]);
+    const float log_q = (t.q[k] - m) * inv - log_s;
+    t.log_q[k] = log_q;
+    t.q[k] = t.ids[k] >= 0 && !none ? exp2_hw(log_q * kLog2e) : 0.f;
+    if (OWNERS && t.ids[k] >= 0) {
+      const int id = t.ids[k], full = a.in.vocab / N;
+      t.next[k] = atomicExch(&t.head[id < full * N ? id / N % THREADS : id - full * N], k);
     }
   }
   __syncthreads();
-  if (empty) return;
-  for (int k = threadIdx.x; k < a.k; k += THREADS) {
-    const int id = t.ids[k], at = id - lo;
-    if (id < 0 || at < 0 || at >= n) continue;
-    float q = 0.f;
-    for (int j = 0; j < a.k; ++j) q += t.ids[j] == id ? t.q[j] : 0.f;      // the same token named twice counts twice
-    out[at] = Elem<DT>::put(gradient(Elem<DT>::get(p[at])) - w * q);
-  }
+  if (OWNERS)
+    for (int k = threadIdx.x; k < a.k; k += THREADS) {
+      float sum = 0.f;
+      for (int j = 0; j < a.k; ++j) sum += t.ids[j] == t.ids[k] ? t.q[j] : 0.f;
+      t.sum[k] = sum;
+    }
+  return none ? 0.f : 1.f;
 }
 
-// A row to a workgroup: its sums, the loss, and with GRAD the gradient from a second reading.
-template <int DT, int THREADS, bool GRAD> __global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
-  __shared__ float lds[THREADS / 64];
-  __shared__ Teacher teacher;
-  const int64_t row = blockIdx.x;
-  const auto* p = static_cast<const typename Elem<DT>::T*>(a.in.z) + row * a.in.stride;
+template <int DT> __device__ inline float student(const DistillArgs& a, int64_t row, int id) {
+  return id >= 0 ? Elem<DT>::get(static_cast<const typename Elem<DT>::T*>(a.in.z)[row * a.in.stride + id]) : 0.f;
+}
+
+// The threads' sums of a row as one, and the row's loss and statistics reported:
+// T^2 sum_k q_k (log q_k - log p_(id_k)), the sum without log S taken along with S itself.
+// `zk`: the student's logit of the thread's first entry.
+template <int DT, int THREADS>
+__device__ inline RowSums join_and_report(const DistillArgs& a, int64_t row, RowSums mine, float zk, float total, const Teacher& t, float* lds) {
   const float c2 = a.in.scale * kLog2e;
-  const RowSums r = join_row<THREADS, false>(sum_row<DT, THREADS, false>(p, a.in.vocab, c2), c2, lds);
+  RowSums r;
+  r.largest = block_max<THREADS>(mine.largest, lds);
+  r.m = fmaxf(r.largest, kLowest);
+  rebase<false>(mine, r.m, c2);
+  r.s = mine.s;
   float kl = 0.f;
-  const float total = load_teacher<THREADS>(a, row, teacher, lds, &r, &kl);
+  for (int k = threadIdx.x; k < a.k; k += THREADS) {
+    const float q = t.q[k], z = k < THREADS ? zk : student<DT>(a, row, t.ids[k]);
+    t.z[k] = z;
+    if (q != 0.f) kl += q * (t.log_q[k] - (z - r.m) * a.in.scale);
+  }
+  block_sum<THREADS>(r.s, kl, lds);
   if (threadIdx.x == 0) {
+    const float log_s = log2_hw(r.s) * kLn2;
+    if (r.s == 0.f) kl = total != 0.f ? INFINITY : 0.f;
+    else kl += total * log_s;
     a.loss[row] = kl * a.temperature * a.temperature;
     a.norm[2 * row] = r.largest;
-    a.norm[2 * row + 1] = log2_hw(r.s) * kLn2;
+    a.norm[2 * row + 1] = log_s;
   }
+  return r;
+}
+
+// dz_i = w T (Q p_i - sum_{k: id_k = i} q_k) with p_i = exp2(c2 (z_i - m) - log2 S).
+struct Gradient {
+  float w, coef, m, c2, shift;
+  __device__ Gradient(const DistillArgs& a, int64_t row, float m_, float log2_s, bool empty, float total)
+      : w(empty ? 0.f : (a.weight ? a.weight[row] : 1.f) * a.temperature), coef(empty ? 0.f : w * total), m(empty ? INFINITY : m_),
+        c2(a.in.scale * kLog2e), shift(empty ? 0.f : log2_s) {}
+  // from the pair that the loss left
+  __device__ Gradient(const DistillArgs& a, int64_t row, float total)
+      : Gradient(a, row, a.norm[2 * row], a.norm[2 * row + 1] * kLog2e, a.norm[2 * row] == -INFINITY && a.norm[2 * row + 1] == -INFINITY, total) {}
+  __device__ float operator()(float z) const { return coef * exp2_hw(__builtin_fmaf(z - m, c2, -shift)); }
+};
+
+// The entries that the teacher names, by the threads that have written those elements without them: a
+// thread's stores to one address stay in order.
+template <int DT>
+__device__ inline void write_named(const Teacher& t, const Gradient& g, typename Elem<DT>::T* out) {
+  for (int k = t.head[threadIdx.x]; k >= 0; k = t.next[k]) out[t.ids[k]] = Elem<DT>::put(g(t.z[k]) - g.w * t.sum[k]);
+}
+
+// A row to a workgroup, in its registers (THREADS * NV vectors) from one reading: the loss and the
+// gradient.  What concerns the teacher is found while the logits arrive.  Bound by memory, with one
+// row of 250 KB on a compute unit by the waits between its reading and its writing too: 8192 x 128000
+// bf16 in 820 us (5.1 TB/s).  Read a second time instead: 1280 us with four times as many rows on the
+// way as the last-level cache holds, 950 us with as many as it does hold.
+template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillArgs a) {
+  constexpr int N = Elem<DT>::N;
+  typedef typename Elem<DT>::T T;
+  __shared__ float lds[2 * THREADS / 64];
+  const Teacher teacher(teacher_lds, a.k);
+  const int64_t row = blockIdx.x;
+  const int n = a.in.vocab, full = n / N, rest = n % N;
+  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride;
+  T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+  const Entry first(a, row, threadIdx.x);
+  u32x4 v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = i * THREADS + static_cast<int>(threadIdx.x);
+    v[i] = u32x4{Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity};
+    if (at < full) v[i] = load16(p + at * N);
+  }
+  const bool tail = static_cast<int>(threadIdx.x) < rest;
+  const float last = tail ? Elem<DT>::get(p[full * N + threadIdx.x]) : -INFINITY;
+  const float zk = student<DT>(a, row, first.id);
+  const float total = load_teacher<THREADS, N, true>(a, row, first, teacher, lds);
+  const float c2 = a.in.scale * kLog2e;
+  RowSums mine;
+#pragma unroll
+  for (int i = 0; i < NV; i += 2) {
+    if (i * THREADS >= full) break;
+    float z[2 * N];
+    Elem<DT>::unpack(v[i], z);
+    Elem<DT>::unpack(v[i + 1], z + N);
+    add_elements<2 * N, false>(mine, z, c2);
+  }
+  const float z[4] = {last, -INFINITY, -INFINITY, -INFINITY};
+  add_elements<4, false>(mine, z, c2);
+  const RowSums r = join_and_report<DT, THREADS>(a, row, mine, zk, total, teacher, lds);
+  const Gradient gradient(a, row, r.m, log2_hw(r.s), r.s == 0.f, total);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS >= full) break;
+    const int at = i * THREADS + static_cast<int>(threadIdx.x);
+    float z[N];
+    Elem<DT>::unpack(v[i], z);
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
+    if (at < full) store16(out + at * N, Elem<DT>::pack(z));
+  }
+  if (tail) out[full * N + threadIdx.x] = Elem<DT>::put(gradient(last));
+  write_named<DT>(teacher, gradient, out);
+}
+
+// The gradient from the pair (m, log S) that the loss left, in two launches: all elements as if the
+// teacher named none of them, a vector a thread in memory order, then a workgroup a row for those
+// that it does name (and for rows where it names none at all, whose gradient is 0).
+template <int DT> __global__ __launch_bounds__(256) void distill_stream(DistillArgs a, int spans) {
+  constexpr int N = Elem<DT>::N;
+  typedef typename Elem<DT>::T T;
+  const int64_t row = blockIdx.x / spans;
+  const int at = (static_cast<int>(blockIdx.x % spans) * 256 + static_cast<int>(threadIdx.x)) * N, n = a.in.vocab - at;
+  if (n <= 0) return;
+  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride + at;
+  T* out = static_cast<T*>(a.grad) + row * a.grad_stride + at;
+  float z[N];
+  if (n >= N) {
+    Elem<DT>::unpack(load16(p), z);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = j < n ? Elem<DT>::get(p[j]) : 0.f;
+  }
+  const Gradient gradient(a, row, 1.f);
+#pragma unroll
+  for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
+  if (n >= N) {
+    stream16(out, Elem<DT>::pack(z));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) out[j] = Elem<DT>::put(z[j]);
+  }
+}
+template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distill_named(DistillArgs a) {
+  __shared__ float lds[THREADS / 64];
+  const Teacher teacher(teacher_lds, a.k);
+  const int64_t row = blockIdx.x;
+  const Entry first(a, row, threadIdx.x);
+  const float zk = student<DT>(a, row, first.id);
+  const float total = load_teacher<THREADS, Elem<DT>::N, true>(a, row, first, teacher, lds);
+  const Gradient gradient(a, row, total);
+  auto* out = static_cast<typename Elem<DT>::T*>(a.grad) + row * a.grad_stride;
+  if (total == 0.f) {
+    for (int i = threadIdx.x; i < a.in.vocab; i += THREADS) out[i] = Elem<DT>::put(0.f);
+    return;
+  }
+  for (int k = threadIdx.x; k < a.k; k += THREADS)
+    if (const int id = teacher.ids[k]; id >= 0)
+      out[id] = Elem<DT>::put(gradient(k < THREADS ? zk : student<DT>(a, row, id)) - gradient.w * teacher.sum[k]);
+}
+
+// The loss alone, or (GRAD) rows longer than a workgroup's registers hold: a second reading.
+template <int DT, int THREADS, bool GRAD> __global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
+  constexpr int N = Elem<DT>::N, U = 4;
+  typedef typename Elem<DT>::T T;
+  __shared__ float lds[2 * THREADS / 64];
+  const Teacher teacher(teacher_lds, a.k);
+  const int64_t row = blockIdx.x;
+  const int n = a.in.vocab;
+  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride;
+  const Entry first(a, row, threadIdx.x);
+  const float zk = student<DT>(a, row, first.id);
+  const float total = load_teacher<THREADS, N, GRAD>(a, row, first, teacher, lds);
+  const RowSums r = join_and_report<DT, THREADS>(a, row, sum_row<DT, THREADS, false>(Segment<DT>(p, n), a.in.scale * kLog2e), zk, total, teacher, lds);
   if constexpr (GRAD) {
-    const float w = (a.weight ? a.weight[row] : 1.f) * a.temperature;
-    write_gradient<DT, THREADS>(a, row, 0, a.in.vocab, r.m, log2_hw(r.s), r.s == 0.f, w, total, teacher);
+    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    const Gradient gradient(a, row, r.m, log2_hw(r.s), r.s == 0.f, total);
+    const int full = n / N;
+    for (int i = threadIdx.x; i < full; i += U * THREADS) {
+      u32x4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * THREADS < full) v[u] = load16(p + static_cast<int64_t>(i + u * THREADS) * N);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u * THREADS >= full) break;
+        float z[N];
+        Elem<DT>::unpack(v[u], z);
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
+        store16(out + static_cast<int64_t>(i + u * THREADS) * N, Elem<DT>::pack(z));
+      }
+    }
+    const int at = full * N + static_cast<int>(threadIdx.x);
+    if (at < n) out[at] = Elem<DT>::put(gradient(Elem<DT>::get(p[at])));
+    write_named<DT>(teacher, gradient, out);
   }
 }
 
-// Few rows: segments' sums, then a workgroup a row joins them and finds the loss.
+// Few rows that are long: segments' sums, then a workgroup a row joins them and finds the loss.
 template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distill_parts(DistillArgs a) {
   __shared__ float lds[THREADS / 64];
   const int64_t row = blockIdx.x / a.split.segs;
   const int lo = static_cast<int>(blockIdx.x % a.split.segs) * a.split.seg, n = min(a.split.seg, a.in.vocab - lo);
   const auto* p = static_cast<const typename Elem<DT>::T*>(a.in.z) + row * a.in.stride + lo;
   const float c2 = a.in.scale * kLog2e;
-  const RowSums r = join_row<THREADS, false>(sum_row<DT, THREADS, false>(p, n, c2), c2, lds);
+  const RowSums r = join_row<THREADS, false>(sum_row<DT, THREADS, false>(Segment<DT>(p, n), c2), c2, lds);
   if (threadIdx.x == 0) static_cast<Partial*>(a.workspace)[blockIdx.x] = {r.largest, r.s, 0.f, 0.f};
 }
-template <int THREADS> __global__ __launch_bounds__(THREADS) void distill_join(DistillArgs a) {
-  __shared__ float lds[THREADS / 64];
-  __shared__ Teacher teacher;
+template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distill_join(DistillArgs a) {
+  __shared__ float lds[2 * THREADS / 64];
+  const Teacher teacher(teacher_lds, a.k);
   const int64_t row = blockIdx.x;
-  const RowSums r = join_parts<THREADS, false>(static_cast<const Partial*>(a.workspace) + row * a.split.segs, a.split.segs,
-                                               a.in.scale * kLog2e, lds);
-  float kl = 0.f;
-  load_teacher<THREADS>(a, row, teacher, lds, &r, &kl);
-  if (threadIdx.x == 0) {
-    a.loss[row] = kl * a.temperature * a.temperature;
-    a.norm[2 * row] = r.largest;
-    a.norm[2 * row + 1] = log2_hw(r.s) * kLn2;
-  }
-}
-
-// The gradient from the pair (m, log S) that the loss left, a workgroup for `span` elements of a row.
-template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distill_grad_rows(DistillArgs a, int spans, int span) {
-  __shared__ float lds[THREADS / 64];
-  __shared__ Teacher teacher;
-  const int64_t row = blockIdx.x / spans;
-  const int lo = static_cast<int>(blockIdx.x % spans) * span, n = min(span, a.in.vocab - lo);
-  const float total = load_teacher<THREADS>(a, row, teacher, lds, nullptr, nullptr);
-  const float m = a.norm[2 * row], log_s = a.norm[2 * row + 1];
-  const bool empty = m == -INFINITY && log_s == -INFINITY;
-  const float w = (a.weight ? a.weight[row] : 1.f) * a.temperature;
-  write_gradient<DT, THREADS>(a, row, lo, n, m, log_s * kLog2e, empty, w, total, teacher);
+  const Entry first(a, row, threadIdx.x);
+  const float zk = student<DT>(a, row, first.id);
+  const float total = load_teacher<THREADS, Elem<DT>::N, false>(a, row, first, teacher, lds);
+  const RowSums mine = add_parts<THREADS, false>(static_cast<const Partial*>(a.workspace) + row * a.split.segs, a.split.segs, a.in.scale * kLog2e);
+  join_and_report<DT, THREADS>(a, row, mine, zk, total, teacher, lds);
 }
 
 template <class F> hipError_t by_type(int dtype, F&& f) {
@@ -527,93 +723,97 @@ template <class F> hipError_t by_type(int dtype, F&& f) {
     default: return f(std::integral_constant<int, kF16>{});
   }
 }
+template <class F> hipError_t by_threads(int threads, F&& f) {
+  switch (threads) {
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    case 256: return f(std::integral_constant<int, 256>{});
+    case 512: return f(std::integral_constant<int, 512>{});
+    default: return f(std::integral_constant<int, 1024>{});
+  }
+}
+unsigned grid_of(int64_t n) { return static_cast<unsigned>(n); }
 
-// `span` elements a workgroup writes of a row, a multiple of a vector; whole rows where that fills
-// the device.
-void spans_of(int64_t rows, int vocab, int dtype, int compute_units, int* spans, int* span) {
-  const RowSplit s = split_rows(rows, vocab, dtype, compute_units);
-  *spans = s.segs;
-  *span = s.seg;
+template <int DT> hipError_t launch_gradient_alone(const DistillArgs& a, hipStream_t stream) {
+  constexpr int span = 256 * Elem<DT>::N;
+  const int spans = (a.in.vocab + span - 1) / span;
+  distill_stream<DT><<<grid_of(a.in.rows * spans), 256, 0, stream>>>(a, spans);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.k <= 64) distill_named<DT, 64><<<grid_of(a.in.rows), 64, Teacher::bytes(a.k, 64), stream>>>(a);
+  else distill_named<DT, 256><<<grid_of(a.in.rows), 256, Teacher::bytes(a.k, 256), stream>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-RowSplit split_rows(int64_t rows, int vocab, int dtype, int compute_units) {
-  const int vec = 16 / static_cast<int>(elem_size(dtype));
-  const int64_t want = 4 * static_cast<int64_t>(compute_units);
-  if (rows >= want) return {1, vocab};
-  // at least two rounds of 256 threads for a segment: below that its fixed costs are the larger part
-  const int64_t least = 2 * 256 * vec;
-  int64_t segs = (want + rows - 1) / rows;
-  segs = segs < (vocab + least - 1) / least ? segs : (vocab + least - 1) / least;
-  if (segs <= 1) return {1, vocab};
-  int64_t seg = (vocab + segs - 1) / segs;
-  seg = (seg + vec - 1) / vec * vec;
-  segs = (vocab + seg - 1) / seg;
-  if (segs <= 1) return {1, vocab};
-  return {static_cast<int>(segs), static_cast<int>(seg)};
-}
-
-size_t split_workspace(const RowSplit& s, int64_t rows, int top) {
-  if (s.segs == 1) return 0;
-  return static_cast<size_t>(rows) * static_cast<size_t>(s.segs) * (sizeof(Partial) + sizeof(uint64_t) * static_cast<size_t>(top));
-}
-
 hipError_t launch_score(const ScoreArgs& a, hipStream_t stream) {
-  constexpr int THREADS = 256;
-  const dim3 grid(static_cast<unsigned>(a.in.rows * a.split.segs));
-  auto both = [&](auto dt, auto ent, auto top) {
-    score_rows<dt.value, THREADS, ent.value, top.value><<<grid, THREADS, 0, stream>>>(a);
-    hipError_t e = hipGetLastError();
+  auto go = [&](auto dt, auto ent, auto top) {
+    hipError_t e = by_threads(a.split.threads, [&](auto threads) {
+      score_rows<dt.value, threads.value, ent.value, top.value><<<grid_of(a.in.rows * a.split.segs), threads.value, 0, stream>>>(a);
+      return hipGetLastError();
+    });
     if (e != hipSuccess || a.split.segs == 1) return e;
-    score_join<THREADS, ent.value, top.value><<<dim3(static_cast<unsigned>(a.in.rows)), THREADS, 0, stream>>>(a);
+    score_join<256, ent.value, top.value><<<grid_of(a.in.rows), 256, 0, stream>>>(a);
     return hipGetLastError();
   };
   return by_type(a.in.dtype, [&](auto dt) {
     const std::true_type yes;
     const std::false_type no;
-    if (a.entropy) return a.top ? both(dt, yes, yes) : both(dt, yes, no);
-    return a.top ? both(dt, no, yes) : both(dt, no, no);
+    if (a.entropy) return a.top ? go(dt, yes, yes) : go(dt, yes, no);
+    return a.top ? go(dt, no, yes) : go(dt, no, no);
   });
 }
 
-hipError_t launch_score_grad(const ScoreGradArgs& a, int compute_units, hipStream_t stream) {
-  int spans, span;
-  spans_of(a.in.rows, a.in.vocab, a.in.dtype, compute_units, &spans, &span);
-  const dim3 grid(static_cast<unsigned>(a.in.rows * spans));
+hipError_t launch_score_grad(const ScoreGradArgs& a, hipStream_t stream) {
   return by_type(a.in.dtype, [&](auto dt) {
-    if (a.grad_entropy) score_grad_rows<dt.value, true><<<grid, 256, 0, stream>>>(a, spans, span);
-    else score_grad_rows<dt.value, false><<<grid, 256, 0, stream>>>(a, spans, span);
+    constexpr int span = 256 * Elem<dt.value>::N;
+    const int spans = (a.in.vocab + span - 1) / span;
+    if (a.grad_entropy) score_grad_rows<dt.value, true><<<grid_of(a.in.rows * spans), 256, 0, stream>>>(a, spans);
+    else score_grad_rows<dt.value, false><<<grid_of(a.in.rows * spans), 256, 0, stream>>>(a, spans);
     return hipGetLastError();
   });
 }
 
-hipError_t launch_distill_grad(const DistillArgs& a, int compute_units, hipStream_t stream) {
-  int spans, span;
-  spans_of(a.in.rows, a.in.vocab, a.in.dtype, compute_units, &spans, &span);
-  const dim3 grid(static_cast<unsigned>(a.in.rows * spans));
-  return by_type(a.in.dtype, [&](auto dt) {
-    distill_grad_rows<dt.value, 256><<<grid, 256, 0, stream>>>(a, spans, span);
-    return hipGetLastError();
-  });
+hipError_t launch_distill_grad(const DistillArgs& a, hipStream_t stream) {
+  return by_type(a.in.dtype, [&](auto dt) { return launch_gradient_alone<dt.value>(a, stream); });
 }
 
-hipError_t launch_distill(const DistillArgs& a, int compute_units, hipStream_t stream) {
-  constexpr int THREADS = 256;
+hipError_t launch_distill(const DistillArgs& a, hipStream_t stream) {
   return by_type(a.in.dtype, [&](auto dt) {
-    const dim3 rows(static_cast<unsigned>(a.in.rows));
-    if (a.split.segs == 1) {
-      if (a.grad) distill_rows<dt.value, THREADS, true><<<rows, THREADS, 0, stream>>>(a);
-      else distill_rows<dt.value, THREADS, false><<<rows, THREADS, 0, stream>>>(a);
-      return hipGetLastError();
+    constexpr int DT = dt.value;
+    const unsigned rows = grid_of(a.in.rows);
+    if (a.split.segs > 1) {
+      distill_parts<DT, 512><<<grid_of(a.in.rows * a.split.segs), 512, 0, stream>>>(a);
+      if (hipError_t e = hipGetLastError()) return e;
+      distill_join<DT, 256><<<rows, 256, Teacher::bytes(a.k, 256), stream>>>(a);
+      hipError_t e = hipGetLastError();
+      return e != hipSuccess || !a.grad ? e : launch_gradient_alone<DT>(a, stream);
     }
-    distill_parts<dt.value, THREADS><<<dim3(static_cast<unsigned>(a.in.rows * a.split.segs)), THREADS, 0, stream>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    distill_join<THREADS><<<rows, THREADS, 0, stream>>>(a);
-    e = hipGetLastError();
-    if (e != hipSuccess || !a.grad) return e;
-    return launch_distill_grad(a, compute_units, stream);
+    if (!a.grad)
+      return by_threads(a.split.threads, [&](auto threads) {
+        distill_rows<DT, threads.value, false><<<rows, threads.value, Teacher::bytes(a.k, threads.value), stream>>>(a);
+        return hipGetLastError();
+      });
+    auto held = [&](auto threads, auto nv) {
+      distill_held<DT, threads.value, nv.value><<<rows, threads.value, Teacher::bytes(a.k, threads.value), stream>>>(a);
+      return hipGetLastError();
+    };
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 16> sixteen;
+    const std::integral_constant<int, 256> t256;
+    const std::integral_constant<int, 1024> t1024;
+    if (a.held.vectors == 4) {
+      if (a.held.threads == 64) return held(std::integral_constant<int, 64>{}, four);
+      if (a.held.threads == 256) return held(t256, four);
+      return held(t1024, four);
+    }
+    if (a.held.vectors == 16) {
+      if (a.held.threads == 256) return held(t256, sixteen);
+      if (a.held.threads == 512) return held(std::integral_constant<int, 512>{}, sixteen);
+      return held(t1024, sixteen);
+    }
+    distill_rows<DT, 1024, true><<<rows, 1024, Teacher::bytes(a.k, 1024), stream>>>(a);
+    return hipGetLastError();
   });
 }
 

@@ -1,0 +1,72 @@
+// How the language-model operators' launches are cut: rules on sizes and types alone.
+#include <algorithm>
+
+#include "operators.hpp"
+
+namespace eh {
+
+// Measured on 256 compute units, us a call:
+//   few rows                     many rows, short                       many rows, long
+//   8 x 32000 bf16               16384 x 1000 bf16                      4096 x 50264 bf16, 20 alternatives
+//   256 threads 11.2, 1024 10.6   64 threads 10.3, 128 13.0, 256 20      256 threads 105, 512 96, 1024 175
+// and 1021 x 50257 f16 with 5: 256 threads 27, 512 34 (its workgroups are all on the device at once, more
+// threads only lengthen the selection).  Segments only pay where a row is long and there are few:
+// 1 x 150000 f32 11.7 against 15.6 with one workgroup of 1024, 64 x 150000 bf16 16.6 against 17.8.
+RowSplit split_rows(int64_t rows, int vocab, int dtype, int compute_units) {
+  const int vec = 16 / static_cast<int>(elem_size(dtype));
+  const int64_t items = (vocab + vec - 1) / vec;
+  if (items > 32768 && rows * 4 <= compute_units) {
+    // 32 KB a segment at least, four vectors for each of 512 threads
+    const int64_t want = (2 * static_cast<int64_t>(compute_units) + rows - 1) / rows;
+    const int64_t segs = std::min<int64_t>(want, items / 2048);
+    const int64_t seg = (items + segs - 1) / segs * vec;
+    return {512, static_cast<int>((vocab + seg - 1) / seg), static_cast<int>(seg)};
+  }
+  if (rows <= compute_units) return {items <= 256 ? 64 : items <= 512 ? 128 : items <= 1024 ? 256 : items <= 2048 ? 512 : 1024, 1, vocab};
+  if (items <= 512) return {64, 1, vocab};
+  if (items <= 2048) return {128, 1, vocab};
+  return {items > 4096 && rows >= 8 * static_cast<int64_t>(compute_units) ? 512 : 256, 1, vocab};
+}
+
+size_t split_workspace(const RowSplit& s, int64_t rows, int top) {
+  if (s.segs == 1) return 0;
+  return static_cast<size_t>(rows) * static_cast<size_t>(s.segs) * (sizeof(RowPartial) + 8 * static_cast<size_t>(top));
+}
+
+// The smallest workgroup that holds a row, with few rows the largest (us a call):
+//   16384 x 1000 bf16     64 x 4 20.9, 256 x 4 49         4096 x 64000 bf16   512 x 16 204, 1024 x 16 245
+//   4096 x 32000 bf16    256 x 16 108, 1024 x 16 156      256 x 32000 bf16    1024 x 4 11.9, 256 x 16 13.8
+RowHeld hold_rows(int64_t rows, int vocab, int dtype, int compute_units) {
+  const int64_t vectors = vocab / (16 / static_cast<int64_t>(elem_size(dtype)));
+  if (vectors <= 256) return {64, 4};
+  if (rows <= 2 * static_cast<int64_t>(compute_units) && vectors <= 4096) return {1024, 4};
+  if (vectors <= 1024) return {256, 4};
+  if (vectors <= 4096) return {256, 16};
+  if (vectors <= 8192) return {512, 16};
+  if (vectors <= 16384) return {1024, 16};
+  return {1024, 0};
+}
+
+ScanPlan plan_scan(const ScanArgs& a) {
+  ScanPlan p{};
+  int64_t step = 0;
+  for (int64_t s : {a.gate.step, a.x.step, a.out.step, a.grad_gate.step, a.grad_x.step}) step = std::max(step, s);
+  p.far = step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 + 1) >= (int64_t{1} << 32);
+  p.waves = p.far ? 8 : a.time <= 64 ? 1 : a.time <= 256 ? 4 : 8;
+  const int64_t piece = p.waves * (64 / kScanLanes) * kScanSteps;
+  p.channels = kScanLanes * (16 / static_cast<int>(elem_size(a.dtype)));
+  p.pieces = std::max<int64_t>((a.time + piece - 1) / piece, 1);
+  p.tiles = (a.width + p.channels - 1) / p.channels;
+  p.per_group = 64 * p.waves / p.channels;
+  p.groups = (p.pieces + p.per_group - 1) / p.per_group;
+  return p;
+}
+
+size_t scan_workspace(const ScanArgs& a) {
+  const ScanPlan p = plan_scan(a);
+  if (p.pieces == 1) return 0;
+  return kTicketBytes + static_cast<size_t>(a.batch * p.tiles) * static_cast<size_t>(p.channels) *
+                            (8 * static_cast<size_t>(p.pieces) + 4 * static_cast<size_t>(p.groups));
+}
+
+}  // namespace eh

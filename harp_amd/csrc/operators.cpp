@@ -224,6 +224,8 @@ void launched(hipError_t e, const char* what) {
 void check_rows(int64_t rows, int64_t vocab) {
   if (rows < 0 || rows > (int64_t{1} << 24)) throw Error("rows: " + std::to_string(rows) + " is out of range (0 to 2^24)");
   if (vocab < 1 || vocab > (int64_t{1} << 30)) throw Error("vocab: " + std::to_string(vocab) + " is out of range (1 to 2^30)");
+  // a launch has a workgroup for every 4 KB of a row
+  if (rows * ((vocab + 1023) / 1024) >= (int64_t{1} << 31)) throw Error("rows, vocab: " + std::to_string(rows) + " rows of " + std::to_string(vocab) + " are out of range together");
 }
 float check_scale(double scale, const char* name) {
   const float f = static_cast<float>(scale);
@@ -243,7 +245,7 @@ int units(const HipDevice& d) { return std::max(d.profile().compute_units, 1); }
 // Float logits may be given with an element type of their own; nothing else decides the split.
 RowSplit split_of(const HipDevice& d, int64_t rows, int64_t vocab, const eh_array& logits) {
   if (!is_float(logits.dtype)) throw Error("logits: has to be f32, bf16 or f16");
-  if (rows == 0) return {1, static_cast<int>(vocab)};
+  if (rows == 0) return {64, 1, static_cast<int>(vocab)};
   return split_rows(rows, static_cast<int>(vocab), static_cast<int>(logits.dtype), units(d));
 }
 
@@ -341,7 +343,7 @@ int eh_token_logprobs_backward(eh_device* dev, const eh_token_logprobs_backward_
     s.grad = arrays.floats("grad", a.grad, a.rows, 1, a.vocab, a.logits.dtype, true);
     s.grad_stride = a.grad.stride[0];
     arrays.settle();
-    if (a.rows) launched(launch_score_grad(s, units(*d), d->stream()), "launch of token_logprobs_backward");
+    if (a.rows) launched(launch_score_grad(s, d->stream()), "launch of token_logprobs_backward");
     arrays.written();
     if (sync) d->synchronize();
   });
@@ -379,13 +381,14 @@ static void distill(eh_device* dev, const eh_distill_loss_args& a, bool backward
     s.grad_stride = a.grad.stride[0];
   }
   s.split = split_of(*d, a.rows, a.vocab, a.logits);
+  s.held = hold_rows(a.rows, s.in.vocab, s.in.dtype, units(*d));
   const eh_array none{};
   Workspace ws(d, arrays, backward ? none : a.workspace, backward ? 0 : split_workspace(s.split, a.rows, 0));
   s.workspace = ws.at();
   arrays.settle();
   if (a.rows) {
-    if (backward) launched(launch_distill_grad(s, units(*d), d->stream()), "launch of distill_loss_backward");
-    else launched(launch_distill(s, units(*d), d->stream()), "launch of distill_loss");
+    if (backward) launched(launch_distill_grad(s, d->stream()), "launch of distill_loss_backward");
+    else launched(launch_distill(s, d->stream()), "launch of distill_loss");
   }
   arrays.written();
 }
@@ -413,20 +416,23 @@ static ScanArgs scan_sizes(int64_t batch, int64_t time, int64_t width, int64_t l
   s.batch = batch, s.time = time, s.width = static_cast<int>(width);
   s.dtype = static_cast<int>(gate.dtype);
   s.log_gate = log_gate != 0;
+  const ScanPlan p = plan_scan(s);
+  if (p.pieces > (int64_t{1} << 31) / std::max<int64_t>(batch * p.tiles, 1))
+    throw Error("batch, time, width: " + std::to_string(batch) + " sequences of " + std::to_string(time) + " steps of " + std::to_string(width) + " channels are out of range together");
   return s;
 }
 
 int eh_gated_scan_workspace(eh_device* dev, const eh_gated_scan_args* args, size_t* bytes) {
   REQUIRE(dev && args && bytes, "device, args or bytes is NULL");
   return guard([&] {
-    *bytes = scan_workspace(scan_sizes(args->batch, args->time, args->width, args->log_gate, args->gate), units(dev->dev));
+    *bytes = scan_workspace(scan_sizes(args->batch, args->time, args->width, args->log_gate, args->gate));
   });
 }
 
 int eh_gated_scan_backward_workspace(eh_device* dev, const eh_gated_scan_backward_args* args, size_t* bytes) {
   REQUIRE(dev && args && bytes, "device, args or bytes is NULL");
   return guard([&] {
-    *bytes = scan_workspace(scan_sizes(args->batch, args->time, args->width, args->log_gate, args->gate), units(dev->dev));
+    *bytes = scan_workspace(scan_sizes(args->batch, args->time, args->width, args->log_gate, args->gate));
   });
 }
 
@@ -446,10 +452,10 @@ int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync) {
     s.state = arrays.small<const float>("state", a.state, a.batch, a.width, EH_F32, false, false);
     s.final_state = arrays.small<float>("final_state", a.final_state, a.batch, a.width, EH_F32, false, true);
     s.lengths = arrays.small<const int>("lengths", a.lengths, a.batch, 1, EH_I32, false, false);
-    Workspace ws(d, arrays, a.workspace, scan_workspace(s, units(*d)));
+    Workspace ws(d, arrays, a.workspace, scan_workspace(s));
     s.workspace = ws.at();
     arrays.settle();
-    if (a.batch) launched(launch_scan(s, units(*d), d->stream()), "launch of gated_scan");
+    if (a.batch) launched(launch_scan(s, d->stream()), "launch of gated_scan");
     arrays.written();
     if (sync) d->synchronize();
   });
@@ -474,10 +480,10 @@ int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* ar
     s.grad_final = arrays.small<const float>("grad_final", a.grad_final, a.batch, a.width, EH_F32, false, false);
     s.final_state = arrays.small<float>("grad_state", a.grad_state, a.batch, a.width, EH_F32, false, true);
     s.lengths = arrays.small<const int>("lengths", a.lengths, a.batch, 1, EH_I32, false, false);
-    Workspace ws(d, arrays, a.workspace, scan_workspace(s, units(*d)));
+    Workspace ws(d, arrays, a.workspace, scan_workspace(s));
     s.workspace = ws.at();
     arrays.settle();
-    if (a.batch) launched(launch_scan_grad(s, units(*d), d->stream()), "launch of gated_scan_backward");
+    if (a.batch) launched(launch_scan_grad(s, d->stream()), "launch of gated_scan_backward");
     arrays.written();
     if (sync) d->synchronize();
   });

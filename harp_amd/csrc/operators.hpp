@@ -31,14 +31,26 @@ struct TokenIds {
   int wide;                // 64-bit integers
 };
 
-// One row's share of work for a workgroup: `segs` segments of `seg` elements.
+// How a pass over rows that reads each once goes to workgroups: a row to one of `threads` threads, or
+// `segs` segments of `seg` elements with a second launch that joins them.
 struct RowSplit {
+  int threads;
   int segs;
   int seg;
 };
-// Splits rows until the launch fills the device; a whole row (segs == 1) where there are enough.
 RowSplit split_rows(int64_t rows, int vocab, int dtype, int compute_units);
+// What a segment leaves for the join (its best keys, 8 bytes each, follow).
+struct RowPartial {
+  float largest, s, t, pad;
+};
 size_t split_workspace(const RowSplit& s, int64_t rows, int top);   // bytes; 0 for whole rows
+
+// A row held in a workgroup's registers, `vectors` of 16 bytes a thread; 0 vectors: too long for that.
+struct RowHeld {
+  int threads;
+  int vectors;
+};
+RowHeld hold_rows(int64_t rows, int vocab, int dtype, int compute_units);
 
 struct ScoreArgs {
   LogitRows in;
@@ -66,7 +78,7 @@ struct ScoreGradArgs {
   void* grad;
   int64_t grad_stride;
 };
-hipError_t launch_score_grad(const ScoreGradArgs& a, int compute_units, hipStream_t stream);
+hipError_t launch_score_grad(const ScoreGradArgs& a, hipStream_t stream);
 
 struct DistillArgs {
   LogitRows in;                // scale is 1 / temperature
@@ -83,10 +95,11 @@ struct DistillArgs {
   void* grad;                  // null: no gradient
   int64_t grad_stride;
   RowSplit split;
+  RowHeld held;
   void* workspace;
 };
-hipError_t launch_distill(const DistillArgs& a, int compute_units, hipStream_t stream);
-hipError_t launch_distill_grad(const DistillArgs& a, int compute_units, hipStream_t stream);
+hipError_t launch_distill(const DistillArgs& a, hipStream_t stream);
+hipError_t launch_distill_grad(const DistillArgs& a, hipStream_t stream);
 
 // Element (b, t, d) at p + b * batch + t * step + d elements.
 struct Sequences {
@@ -107,8 +120,20 @@ struct ScanArgs {
   const int* lengths;          // [batch] or null
   void* workspace;
 };
-size_t scan_workspace(const ScanArgs& a, int compute_units);
-hipError_t launch_scan(const ScanArgs& a, int compute_units, hipStream_t stream);
-hipError_t launch_scan_grad(const ScanArgs& a, int compute_units, hipStream_t stream);
+// A workgroup of `waves` waves has kScanLanes vectors of channels and a piece of waves * 64 steps.
+constexpr int kScanSteps = 8;        // of a thread
+constexpr int kScanLanes = 8;        // side by side
+struct ScanPlan {
+  int waves;
+  bool far;                          // a piece's rows may lie further apart than 32-bit offsets reach
+  int channels;                      // of a workgroup
+  int64_t pieces, tiles;             // of a sequence, of a row
+  int64_t per_group, groups;         // pieces whose maps are composed from one state
+};
+ScanPlan plan_scan(const ScanArgs& a);
+constexpr size_t kTicketBytes = 256;
+size_t scan_workspace(const ScanArgs& a);     // bytes; 0 where a sequence is one piece
+hipError_t launch_scan(const ScanArgs& a, hipStream_t stream);
+hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t stream);
 
 }  // namespace eh

@@ -85,6 +85,16 @@ def test_score_sizes(dev, ops, n, v, dtype):
     check_score(dev, ops, z, t, top=min(v, 32), scale=1.6)
 
 
+@pytest.mark.parametrize("dtype,n,v", [("f32", 1, 140001), ("bf16", 2, 300003), ("f32", 60, 131080), ("f32", 260, 2001), ("f32", 260, 8003),
+                                       ("f32", 260, 16001), ("bf16", 2050, 33001), ("f16", 70, 270000)])
+def test_score_of_every_launch_shape(dev, ops, dtype, n, v):
+    """Rows of one to sixteen waves, rows in segments, aligned and not."""
+    z = rows_of(n, v, dtype, seed=v)
+    t = on_gpu(np.random.default_rng(5).integers(0, v, n))
+    check_score(dev, ops, z, t, top=20)
+    check_score(dev, ops, z, t, top=0, entropy=False)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,v,shift", [(3, 1001, 1), (5, 4099, 3), (2, 33000, 5)])
 def test_score_rows_at_any_alignment(dev, ops, n, v, shift, dtype):
@@ -230,7 +240,8 @@ def check_distill(dev, ops, z, u, ids, temperature, weight, dtype, workspace=Non
     assert bool((grad[:, v:] == 5.0).all())
     alone = ops.Distilled(torch.empty(n, device="cuda"), torch.empty(n, 2, device="cuda"), None)
     ops.distill_loss(dev, z, u, ids, temperature=temperature, out=alone, workspace=workspace)
-    assert torch.equal(alone.loss, out.loss) and torch.equal(alone.norm, out.norm)
+    close(host(alone.loss), loss, loss_tol, "loss alone")                # (sums in another order than with the gradient)
+    close(host(alone.norm), norm, norm_tol, "norm alone")
     later = ops.distill_loss_backward(dev, z, u, ids, out.norm, w, temperature=temperature, out=torch.full((n, v), 5.0, device="cuda", dtype=DT[dtype]))
     _, _, _, _, want, tol = oracle.distill(host(z), host(u), ids.cpu().numpy(), temperature, weight, norm=host(out.norm))
     close(host(later), want, tol + oracle.rounding(dtype, want), "later gradient")
@@ -238,6 +249,17 @@ def check_distill(dev, ops, z, u, ids, temperature, weight, dtype, workspace=Non
 
 
 DISTILL = [(1, 1, 1), (1, 5, 3), (3, 64, 7), (2, 1000, 100), (6, 2051, 1), (1, 50000, 40), (9, 9000, 257), (3, 1100, 1024), (1030, 97, 5)]
+DISTILL_SHAPES = [("f32", 3, 16001, 30), ("f32", 520, 4001, 3), ("bf16", 520, 16003, 70), ("f32", 520, 32001, 5), ("f32", 3, 60001, 1024), ("bf16", 2, 131075, 65),
+                  ("f32", 70, 70001, 20), ("f16", 2, 140003, 200), ("f32", 2, 140001, 20), ("bf16", 1, 300000, 300)]
+
+
+@pytest.mark.parametrize("dtype,n,v,k", DISTILL_SHAPES)
+def test_distill_of_every_launch_shape(dev, ops, dtype, n, v, k):
+    """Rows held by 64 to 1024 threads, rows read twice, rows in segments."""
+    rng = np.random.default_rng(v + k)
+    ids = rng.integers(0, v, (n, k))
+    ids[:, k // 2:][rng.random((n, k - k // 2)) < 0.3] = v - 1                   # the last element, often
+    check_distill(dev, ops, rows_of(n, v, dtype, seed=v), on_gpu(rng.normal(0, 3, (n, k)).astype(np.float32)), on_gpu(ids), 1.5, rng.random(n).astype(np.float32), dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -484,7 +506,7 @@ def test_no_rows_and_no_steps(dev, ops):
     torch.cuda.synchronize()
 
 
-def _all_calls(dev, ops, seed, n=5, v=20000, k=9, b=2, t=900, d=40):
+def _all_calls(dev, ops, seed, n=5, v=270000, k=9, b=2, t=1300, d=40):
     """One call of each operator on inputs of the seed: (a function that runs them, their outputs, workspaces)."""
     rng = np.random.default_rng(seed)
     z = rows_of(n, v, "bf16", seed)
@@ -584,7 +606,7 @@ def test_capture_needs_the_callers_workspace(ops):
     s = torch.cuda.Stream()
     h = hb.HipDevice(0, stream=s.cuda_stream)
     with torch.cuda.stream(s):
-        z = torch.randn(2, 100000, device="cuda")
+        z = torch.randn(2, 300000, device="cuda")
         t = torch.zeros(2, device="cuda", dtype=torch.int64)
         out = ops.Logprobs(torch.empty(2, device="cuda"), None, torch.empty(2, 2, device="cuda"), None, None)
         assert ops.token_logprobs_workspace(h, z) > 0
