@@ -12,7 +12,7 @@ namespace eh {
 namespace {
 
 constexpr float kLowest = -3.402823466e+38f;
-constexpr int kCandidates = 512;          // elements at or above the selection's threshold that LDS holds
+constexpr int kCandidates = 256;          // elements at or above the selection's threshold that LDS holds
 
 // A segment of a row as items of N elements that start at 16-byte boundaries, whatever the row's own
 // start: item i has elements [N i - skew, N i - skew + N) of the segment, the first and the last item
@@ -125,10 +125,10 @@ __device__ inline float value_of(uint32_t o) { return __uint_as_float(o & 0x8000
 __device__ inline uint64_t key_of(uint32_t order, uint32_t place) { return static_cast<uint64_t>(order) << 32 | (0xffffffffu - place); }
 __device__ inline uint32_t place_of(uint64_t key) { return 0xffffffffu - static_cast<uint32_t>(key); }
 
-struct Selection {
+template <int THREADS> struct Selection {
   uint32_t group[64];
   int count, owners;
-  uint16_t owner[1024];
+  uint16_t owner[THREADS];
   uint64_t found[kCandidates];
   uint64_t top[kMaxTop];
 };
@@ -138,7 +138,7 @@ struct Selection {
 
 // A segment of a row by its items; `base` is the segment's place in its row.
 template <int DT> struct RowSource {
-  static constexpr int N = Elem<DT>::N, U = 4;
+  static constexpr int N = Elem<DT>::N, U = 2;
   Segment<DT> row;
   int base;
   __device__ int items() const { return row.items(); }
@@ -208,7 +208,7 @@ template <int THREADS, class Source, class F> __device__ inline void visit_own(c
 // eight rows on a compute unit).  A wave finds the threshold bit by bit with ballots.  A row with
 // many elements there (equal ones, say) takes k rounds over the row instead.
 template <int THREADS, class Source>
-__device__ inline void select_top(const Source& src, uint32_t mine, int k, Selection& sel) {
+__device__ inline void select_top(const Source& src, uint32_t mine, int k, Selection<THREADS>& sel) {
   constexpr int G = THREADS / 64;
   uint32_t g = mine;
   if (G >= 2) g = max(g, dpp<kSwap1>(g, g));
@@ -292,7 +292,7 @@ struct Target {
 };
 
 // What a row reports, once its sums (and best keys) are known.  All threads of the workgroup call it.
-__device__ inline void report_row(const ScoreArgs& a, int64_t row, const RowSums& r, const Target& target, const Selection* sel) {
+__device__ inline void report_row(const ScoreArgs& a, int64_t row, const RowSums& r, const Target& target, const uint64_t* top) {
   const float scale = a.in.scale;
   const bool empty = r.s == 0.f;                            // no element above -infinity
   const float log_s = log2_hw(r.s) * kLn2;
@@ -310,7 +310,7 @@ __device__ inline void report_row(const ScoreArgs& a, int64_t row, const RowSums
   }
   const int j = threadIdx.x;
   if (a.top && j < a.top) {
-    const uint64_t key = sel->top[j];
+    const uint64_t key = top[j];
     const uint32_t order = static_cast<uint32_t>(key >> 32);
     a.top_ids[row * a.top + j] = static_cast<int>(place_of(key));
     a.top_logp[row * a.top + j] = empty ? -INFINITY : (value_of(order) - r.m) * scale - log_s;
@@ -318,9 +318,9 @@ __device__ inline void report_row(const ScoreArgs& a, int64_t row, const RowSums
 }
 
 // A workgroup for each segment of each row; whole rows are reported at once.
-template <int DT, int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS) void score_rows(ScoreArgs a) {
+template <int DT, int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 4 : THREADS == 64 ? 6 : 8) void score_rows(ScoreArgs a) {
   __shared__ float lds[THREADS / 64];
-  __shared__ typename std::conditional<TOP, Selection, char>::type sel;
+  __shared__ typename std::conditional<TOP, Selection<THREADS>, char>::type sel;
   const int64_t row = blockIdx.x / a.split.segs;
   const int seg = blockIdx.x % a.split.segs, lo = seg * a.split.seg;
   const int n = min(a.split.seg, a.in.vocab - lo);
@@ -341,7 +341,7 @@ template <int DT, int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(
     }
   }
   if (a.split.segs == 1) {
-    if constexpr (TOP) report_row(a, row, r, target, &sel);
+    if constexpr (TOP) report_row(a, row, r, target, sel.top);
     else report_row(a, row, r, target, nullptr);
     return;
   }
@@ -372,7 +372,7 @@ template <int THREADS, bool ENT> __device__ inline RowSums add_parts(const Parti
 
 template <int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS) void score_join(ScoreArgs a) {
   __shared__ float lds[THREADS / 64];
-  __shared__ typename std::conditional<TOP, Selection, char>::type sel;
+  __shared__ typename std::conditional<TOP, Selection<THREADS>, char>::type sel;
   const int64_t row = blockIdx.x;
   const int segs = a.split.segs;
   const Partial* parts = static_cast<const Partial*>(a.workspace);
@@ -384,7 +384,7 @@ template <int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS)
     uint32_t mine = 0;
     visit_own<THREADS>(src, [&](uint32_t order, uint32_t) { mine = max(mine, order); });
     select_top<THREADS>(src, mine, a.top, sel);
-    report_row(a, row, r, target, &sel);
+    report_row(a, row, r, target, sel.top);
   } else {
     report_row(a, row, r, target, nullptr);
   }
