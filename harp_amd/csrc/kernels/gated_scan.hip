@@ -21,11 +21,20 @@ template <int DT> struct Chunk {
 // steps, then 32-bit words of the state behind them.  A word says by itself that it is there: nothing
 // writes the all-ones pattern that the words start with, which is one of NaN's.
 struct Board {
-  unsigned int* ticket;
+  unsigned int* tickets;         // of each class, kTicketStride words apart
   unsigned long long* maps;
   unsigned int* states;
 };
 constexpr unsigned int kEmpty = 0xffffffffu;
+
+constexpr int kTicketStride = 8;
+
+// Class `i` of `classes` into which `n` columns are dealt, in runs of neighbours.
+struct Class {
+  int number;
+  int64_t first, columns;
+  __device__ Class(int64_t n, int classes, int i) : number(i), first(n / classes * i + min(n % classes, int64_t{i})), columns(n / classes + (i < n % classes)) {}
+};
 
 __device__ inline unsigned int word_of(float x) {
   const unsigned int b = __float_as_uint(x);
@@ -111,26 +120,52 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 // steps.  Each leaves its map on the board before it looks at anybody else's, the last of a group the
 // state behind it; a piece composes the state before its group with the maps of the group's pieces
 // before it, all read at once.  Which words are read depends on the piece alone, so results do not
-// depend on the order in which workgroups run.  Workgroups take their pieces from a ticket in the
-// order of the steps: a piece only waits for pieces that have started, for maps that are left without
-// waiting and for the state of the group before, whose waits end for the same reason.
+// depend on the order in which workgroups run.
+//
+// Columns (a sequence's channels of one workgroup's width) are dealt to classes in runs of neighbours;
+// a workgroup takes a ticket of its class, of the next one where that has no pieces left.  A class's
+// pieces go out in the order of the steps, all of a column's in one class: a piece only waits for
+// pieces that have been taken, by workgroups that run, for maps that are left without waiting and for
+// the state of the group before, whose waits end for the same reason.  There are as many workgroups as
+// pieces, so all are taken.
+//
+// With eight classes, by the workgroup's number, neighbouring columns are read and written behind one
+// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes XX us
+// instead of 44 (64 x 512 x 1000 f32 84 instead of 104).  Where they do start there, one class is better
+// (8 x 4096 x 2048 bf16 87 us instead of 91 to 102).
 template <int DT, int W, bool BACK, bool LOG, bool FAR, int EU>
-__global__ __launch_bounds__(64 * W, EU) void scan_chunks(ScanArgs a, int chunks, int tiles, Board board) {
+__global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces, int tiles, int classes, Board board) {
   constexpr int N = Elem<DT>::N, CW = Chunk<DT>::CW, RUN = W * 64 / kLanes * kSteps, P = 64 * W / CW;
   typedef typename Elem<DT>::T T;
   __shared__ float maps[2][W][CW];
   __shared__ float others[2][P][CW];
   __shared__ float before[CW];
-  __shared__ unsigned int turn;
+  __shared__ int64_t turn[2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t columns = a.batch * tiles;
-  int64_t piece = blockIdx.x;
-  if (W == 8 && chunks > 1) {
-    if (threadIdx.x == 0) turn = atomicAdd(board.ticket, 1u) + 1u;       // the word starts at all ones
+  int64_t column, k = 0;
+  if (W == 8 && pieces > 1) {
+    if (threadIdx.x == 0) {
+      turn[0] = -1;
+      for (int i = 0; i < classes; ++i) {
+        const Class c(columns, classes, (blockIdx.x + i) % classes);
+        const unsigned int t = atomicAdd(board.tickets + c.number * kTicketStride, 1u) + 1u;      // the words start at all ones
+        if (t < c.columns * pieces) {
+          turn[0] = c.first + t % c.columns;
+          turn[1] = t / c.columns;
+          break;
+        }
+      }
+    }
     __syncthreads();
-    piece = turn;
+    column = turn[0];
+    k = turn[1];
+    if (column < 0) return;
+  } else {
+    const Class c(columns, classes, blockIdx.x % classes);
+    column = c.first + blockIdx.x / classes;
   }
-  const int64_t column = piece % columns;
+  if (BACK) k = pieces - 1 - k;
   const int64_t b = column / tiles;
   const int tile = static_cast<int>(column % tiles) * CW;
   const int c0 = tile + (lane % kLanes) * N;
@@ -138,7 +173,6 @@ __global__ __launch_bounds__(64 * W, EU) void scan_chunks(ScanArgs a, int chunks
   int64_t n = a.time;
   if (a.lengths) n = min(n, max(static_cast<int64_t>(a.lengths[b]), int64_t{0}));
   const int64_t last = n > 0 ? (n - 1) / RUN : 0;                         // the sequence's last piece
-  const int64_t k = BACK ? chunks - 1 - piece / columns : piece / columns;
   if (k > last) return;
   const int64_t behind = BACK ? last - k : k;                             // pieces before this one, in the order of the steps
   const int run = wave * (64 / kLanes) + lane / kLanes;                   // this thread's place among the runs
@@ -208,9 +242,9 @@ __global__ __launch_bounds__(64 * W, EU) void scan_chunks(ScanArgs a, int chunks
       ma *= maps[0][w][c];
     }
   }
-  const size_t group = static_cast<size_t>(column) * ((chunks + P - 1) / P) + behind / P;
-  if (W == 8 && chunks > 1) {
-    unsigned long long* words = board.maps + (static_cast<size_t>(column) * chunks + behind) * CW + c;
+  const size_t group = static_cast<size_t>(column) * ((pieces + P - 1) / P) + behind / P;
+  if (W == 8 && pieces > 1) {
+    unsigned long long* words = board.maps + (static_cast<size_t>(column) * pieces + behind) * CW + c;
     if (p == 0 && mine && behind < last && member < P - 1)
       __hip_atomic_store(words, static_cast<unsigned long long>(word_of(ma)) << 32 | word_of(mb), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (mine && p < member) {
@@ -295,6 +329,92 @@ __global__ __launch_bounds__(64 * W, EU) void scan_chunks(ScanArgs a, int chunks
   }
 }
 
+// One channel of a short sequence, step by step.
+template <int DT, bool BACK, bool LOG> __device__ inline void scan_channel(const ScanArgs& a, int64_t b, int c, int n) {
+  typedef typename Elem<DT>::T T;
+  auto at = [&](const Sequences& s, int t) { return static_cast<T*>(s.p) + b * s.batch + t * s.step + c; };
+  const int64_t end = b * a.width + c;
+  const float* start = BACK ? a.grad_final : a.state;
+  float h = start ? start[end] : 0.f;
+  for (int s = 0; s < n; ++s) {
+    const int t = BACK ? n - 1 - s : s;
+    float g = Elem<DT>::get(*at(a.gate, t));
+    if (LOG) g = exp2_hw(g * kLog2e);
+    if constexpr (!BACK) {
+      h = __builtin_fmaf(g, h, Elem<DT>::get(*at(a.x, t)));
+      *at(a.out, t) = Elem<DT>::put(h);
+    } else {
+      const float l = Elem<DT>::get(*at(a.out, t)) + h;
+      const float prev = (t > 0 ? Elem<DT>::get(*at(a.x, t - 1)) : a.state ? a.state[end] : 0.f) * l;
+      *at(a.grad_x, t) = Elem<DT>::put(l);
+      *at(a.grad_gate, t) = Elem<DT>::put(LOG ? prev * g : prev);
+      h = g * l;
+    }
+  }
+  if (a.final_state) a.final_state[end] = h;
+}
+
+// Sequences of up to STEPS steps (a decoding step: one), a thread for a vector of channels: all loads
+// first, then the steps.
+template <int DT, int STEPS, bool BACK, bool LOG> __global__ __launch_bounds__(256, 4) void scan_short(ScanArgs a, int vectors) {
+  constexpr int N = Elem<DT>::N;
+  typedef typename Elem<DT>::T T;
+  const int64_t i = blockIdx.x * int64_t{256} + threadIdx.x, b = i / vectors;
+  if (b >= a.batch) return;
+  const int c0 = static_cast<int>(i % vectors) * N;
+  int n = static_cast<int>(a.time);
+  if (a.lengths) n = min(n, max(a.lengths[b], 0));
+  if (a.width - c0 < N) {
+    for (int c = c0; c < a.width; ++c) scan_channel<DT, BACK, LOG>(a, b, c, n);
+    return;
+  }
+  auto row = [&](const Sequences& s, int t) { return static_cast<T*>(s.p) + b * s.batch + t * s.step + c0; };
+  u32x4 vg[STEPS] = {}, vx[STEPS] = {}, vh[STEPS] = {};
+#pragma unroll
+  for (int t = 0; t < STEPS; ++t)
+    if (t < n) {
+      vg[t] = load16(row(a.gate, t));
+      vx[t] = load16(row(BACK ? a.out : a.x, t));
+      if (BACK && t > 0) vh[t] = load16(row(a.x, t - 1));
+    }
+  const int64_t end = b * a.width + c0;
+  auto get = [&](const float* p, float* z) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) Elem<kF32>::unpack(p ? load16(p + end + j) : u32x4{0, 0, 0, 0}, z + j);
+  };
+  float h[N], first[N];
+  get(BACK ? a.grad_final : a.state, h);
+  if (BACK) get(a.state, first);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int t = BACK ? STEPS - 1 - s : s;
+    if (t >= n) continue;
+    float g[N], x[N];
+    step_of<DT, LOG>(vg[t], vx[t], true, g, x);
+    if constexpr (!BACK) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(g[j], h[j], x[j]);
+      store16(row(a.out, t), Elem<DT>::pack(h));
+    } else {
+      float prev[N];
+      if (t > 0) Elem<DT>::unpack(vh[t], prev);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (t == 0) prev[j] = first[j];
+        x[j] += h[j];
+        prev[j] *= x[j];
+        if (LOG) prev[j] *= g[j];
+        h[j] = g[j] * x[j];
+      }
+      store16(row(a.grad_x, t), Elem<DT>::pack(x));
+      store16(row(a.grad_gate, t), Elem<DT>::pack(prev));
+    }
+  }
+  if (!a.final_state) return;
+#pragma unroll
+  for (int j = 0; j < N; j += 4) store16(a.final_state + end + j, Elem<kF32>::pack(h + j));
+}
+
 __global__ __launch_bounds__(256) void clear_board(unsigned int* p, size_t n) {
   for (size_t i = blockIdx.x * size_t{256} + threadIdx.x; i < n; i += size_t{256} * gridDim.x) p[i] = kEmpty;
 }
@@ -309,22 +429,35 @@ template <class F> hipError_t by_type(int dtype, F&& f) {
 
 template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
   const ScanPlan p = plan_scan(a);
+  if (p.waves == 0) {
+    return by_type(a.dtype, [&](auto dt) {
+      const int vectors = (a.width + Elem<dt.value>::N - 1) / Elem<dt.value>::N;
+      const dim3 grid(static_cast<unsigned>((a.batch * vectors + 255) / 256));
+      auto go = [&](auto steps) {
+        if (a.log_gate) scan_short<dt.value, steps.value, BACK, true><<<grid, 256, 0, stream>>>(a, vectors);
+        else scan_short<dt.value, steps.value, BACK, false><<<grid, 256, 0, stream>>>(a, vectors);
+        return hipGetLastError();
+      };
+      if (a.time <= 1) return go(std::integral_constant<int, 1>{});
+      return go(std::integral_constant<int, kSteps>{});
+    });
+  }
   Board board{};
   if (p.pieces > 1) {
     const size_t words = scan_workspace(a) / 4;
-    board.ticket = static_cast<unsigned int*>(a.workspace);
-    board.maps = reinterpret_cast<unsigned long long*>(board.ticket + kTicketBytes / 4);
+    board.tickets = static_cast<unsigned int*>(a.workspace);
+    board.maps = reinterpret_cast<unsigned long long*>(board.tickets + kTicketBytes / 4);
     board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.pieces * p.channels);
     const size_t blocks = (words + 1023) / 1024;
-    clear_board<<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), 256, 0, stream>>>(board.ticket, words);
+    clear_board<<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), 256, 0, stream>>>(board.tickets, words);
     if (hipError_t e = hipGetLastError()) return e;
   }
   const dim3 grid(static_cast<unsigned>(a.batch * p.tiles * p.pieces));
   return by_type(a.dtype, [&](auto dt) {
     auto go = [&](auto waves, auto is_far, auto eu) {
       const int pieces = static_cast<int>(p.pieces), tiles = static_cast<int>(p.tiles);
-      if (a.log_gate) scan_chunks<dt.value, waves.value, BACK, true, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, board);
-      else scan_chunks<dt.value, waves.value, BACK, false, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, board);
+      if (a.log_gate) scan_pieces<dt.value, waves.value, BACK, true, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, p.classes, board);
+      else scan_pieces<dt.value, waves.value, BACK, false, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, p.classes, board);
       return hipGetLastError();
     };
     const std::integral_constant<int, 2> two;

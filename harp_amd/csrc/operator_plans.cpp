@@ -47,18 +47,28 @@ RowHeld hold_rows(int64_t rows, int vocab, int dtype, int compute_units) {
   return {1024, 0};
 }
 
+// Whether every row starts at a cache line.
+static bool on_lines(const Sequences& s, const ScanArgs& a) {
+  const int64_t size = static_cast<int64_t>(elem_size(a.dtype));
+  return reinterpret_cast<uintptr_t>(s.p) % 128 == 0 && (a.time <= 1 || s.step * size % 128 == 0) && (a.batch <= 1 || s.batch * size % 128 == 0);
+}
+
 ScanPlan plan_scan(const ScanArgs& a) {
   ScanPlan p{};
   int64_t step = 0;
   for (int64_t s : {a.gate.step, a.x.step, a.out.step, a.grad_gate.step, a.grad_x.step}) step = std::max(step, s);
   p.far = step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 + 1) >= (int64_t{1} << 32);
-  p.waves = p.far ? 8 : a.time <= 64 ? 1 : a.time <= 256 ? 4 : 8;
-  const int64_t piece = p.waves * (64 / kScanLanes) * kScanSteps;
+  p.waves = a.time <= kScanSteps ? 0 : p.far ? 8 : a.time <= 64 ? 1 : a.time <= 256 ? 4 : 8;
+  const int64_t piece = std::max(p.waves, 1) * (64 / kScanLanes) * kScanSteps;
   p.channels = kScanLanes * (16 / static_cast<int>(elem_size(a.dtype)));
   p.pieces = std::max<int64_t>((a.time + piece - 1) / piece, 1);
   p.tiles = (a.width + p.channels - 1) / p.channels;
-  p.per_group = 64 * p.waves / p.channels;
+  p.per_group = std::max(64 * p.waves / p.channels, 1);
   p.groups = (p.pieces + p.per_group - 1) / p.per_group;
+  bool lines = true;
+  for (const Sequences* s : {&a.gate, &a.x, &a.out, &a.grad_gate, &a.grad_x})
+    if (s->p) lines = lines && on_lines(*s, a);
+  p.classes = lines ? 1 : 8;
   return p;
 }
 

@@ -124,11 +124,12 @@ struct ScanArgs {
 constexpr int kScanSteps = 8;        // of a thread
 constexpr int kScanLanes = 8;        // side by side
 struct ScanPlan {
-  int waves;
+  int waves;                         // 0: a thread has a whole sequence's steps of its channels
   bool far;                          // a piece's rows may lie further apart than 32-bit offsets reach
   int channels;                      // of a workgroup
   int64_t pieces, tiles;             // of a sequence, of a row
   int64_t per_group, groups;         // pieces whose maps are composed from one state
+  int classes;                       // of columns, see the kernel
 };
 ScanPlan plan_scan(const ScanArgs& a);
 constexpr size_t kTicketBytes = 256;
