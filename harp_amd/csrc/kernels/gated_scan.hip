@@ -130,9 +130,11 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 // pieces, so all are taken.
 //
 // With eight classes, by the workgroup's number, neighbouring columns are read and written behind one
-// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes XX us
+// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes 38 us
 // instead of 44 (64 x 512 x 1000 f32 84 instead of 104).  Where they do start there, one class is better
 // (8 x 4096 x 2048 bf16 87 us instead of 91 to 102).
+// a wave has 64 steps, which the plan's choice of waves goes by, and a workgroup a thread per channel
+static_assert(64 / kLanes * kSteps == 64 && kLanes * 8 <= 64);
 template <int DT, int W, bool BACK, bool LOG, bool FAR, int EU>
 __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces, int tiles, int classes, Board board) {
   constexpr int N = Elem<DT>::N, CW = Chunk<DT>::CW, RUN = W * 64 / kLanes * kSteps, P = 64 * W / CW;
@@ -164,6 +166,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
   } else {
     const Class c(columns, classes, blockIdx.x % classes);
     column = c.first + blockIdx.x / classes;
+    if (column >= columns) return;
   }
   if (BACK) k = pieces - 1 - k;
   const int64_t b = column / tiles;
@@ -354,9 +357,9 @@ template <int DT, bool BACK, bool LOG> __device__ inline void scan_channel(const
   if (a.final_state) a.final_state[end] = h;
 }
 
-// Sequences of up to STEPS steps (a decoding step: one), a thread for a vector of channels: all loads
-// first, then the steps.
-template <int DT, int STEPS, bool BACK, bool LOG> __global__ __launch_bounds__(256, 4) void scan_short(ScanArgs a, int vectors) {
+// Short sequences (a decoding step: STEPS = 1), a thread for a vector of channels: the loads of STEPS
+// steps first, then the steps.
+template <int DT, int STEPS, bool BACK, bool LOG> __global__ __launch_bounds__(256, BACK ? 3 : 4) void scan_short(ScanArgs a, int vectors) {
   constexpr int N = Elem<DT>::N;
   typedef typename Elem<DT>::T T;
   const int64_t i = blockIdx.x * int64_t{256} + threadIdx.x, b = i / vectors;
@@ -369,14 +372,6 @@ template <int DT, int STEPS, bool BACK, bool LOG> __global__ __launch_bounds__(2
     return;
   }
   auto row = [&](const Sequences& s, int t) { return static_cast<T*>(s.p) + b * s.batch + t * s.step + c0; };
-  u32x4 vg[STEPS] = {}, vx[STEPS] = {}, vh[STEPS] = {};
-#pragma unroll
-  for (int t = 0; t < STEPS; ++t)
-    if (t < n) {
-      vg[t] = load16(row(a.gate, t));
-      vx[t] = load16(row(BACK ? a.out : a.x, t));
-      if (BACK && t > 0) vh[t] = load16(row(a.x, t - 1));
-    }
   const int64_t end = b * a.width + c0;
   auto get = [&](const float* p, float* z) {
 #pragma unroll
@@ -385,29 +380,41 @@ template <int DT, int STEPS, bool BACK, bool LOG> __global__ __launch_bounds__(2
   float h[N], first[N];
   get(BACK ? a.grad_final : a.state, h);
   if (BACK) get(a.state, first);
+  const int parts = (n + STEPS - 1) / STEPS;
+  for (int part = 0; part < parts; ++part) {
+    const int t0 = (BACK ? parts - 1 - part : part) * STEPS;
+    u32x4 vg[STEPS] = {}, vx[STEPS] = {}, vh[STEPS] = {};
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    const int t = BACK ? STEPS - 1 - s : s;
-    if (t >= n) continue;
-    float g[N], x[N];
-    step_of<DT, LOG>(vg[t], vx[t], true, g, x);
-    if constexpr (!BACK) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(g[j], h[j], x[j]);
-      store16(row(a.out, t), Elem<DT>::pack(h));
-    } else {
-      float prev[N];
-      if (t > 0) Elem<DT>::unpack(vh[t], prev);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (t == 0) prev[j] = first[j];
-        x[j] += h[j];
-        prev[j] *= x[j];
-        if (LOG) prev[j] *= g[j];
-        h[j] = g[j] * x[j];
+    for (int i = 0; i < STEPS; ++i)
+      if (t0 + i < n) {
+        vg[i] = load16(row(a.gate, t0 + i));
+        vx[i] = load16(row(BACK ? a.out : a.x, t0 + i));
+        if (BACK && t0 + i > 0) vh[i] = load16(row(a.x, t0 + i - 1));
       }
-      store16(row(a.grad_x, t), Elem<DT>::pack(x));
-      store16(row(a.grad_gate, t), Elem<DT>::pack(prev));
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int i = BACK ? STEPS - 1 - s : s, t = t0 + i;
+      if (t >= n) continue;
+      float g[N], x[N];
+      step_of<DT, LOG>(vg[i], vx[i], true, g, x);
+      if constexpr (!BACK) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(g[j], h[j], x[j]);
+        store16(row(a.out, t), Elem<DT>::pack(h));
+      } else {
+        float prev[N];
+        Elem<DT>::unpack(vh[i], prev);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (t == 0) prev[j] = first[j];
+          x[j] += h[j];
+          prev[j] *= x[j];
+          if (LOG) prev[j] *= g[j];
+          h[j] = g[j] * x[j];
+        }
+        store16(row(a.grad_x, t), Elem<DT>::pack(x));
+        store16(row(a.grad_gate, t), Elem<DT>::pack(prev));
+      }
     }
   }
   if (!a.final_state) return;
