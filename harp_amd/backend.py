@@ -393,6 +393,10 @@ class HipBackendRegistry:
     def compile_program(self, device: HipDevice, program) -> HipProgram:
         return HipProgram(device, program, self.options)
 
+    def run_operator(self, device: HipDevice, name: str, attrs: dict, inputs, outputs) -> List[HipBuffer]:
+        from . import operators
+        return operators.run(device, name, attrs, inputs, outputs)
+
 
 def init(options=None) -> None:
     """Registers the backend with the front end (the reference crates do this

@@ -143,6 +143,25 @@ def build_host_fuzz(force: bool = False) -> str:
     return FUZZ
 
 
+HOST_CHECKS_SRC = os.path.join(os.path.dirname(HERE), "tests", "operators_host.cpp")
+HOST_CHECKS = os.path.join(os.path.dirname(HERE), "tests", "operators_host.bin")
+
+
+def build_operator_checks(force: bool = False) -> str:
+    """tests/operators_host.cpp: the operators' entry points and plans on stand-ins for the device, built by
+    g++ with AddressSanitizer and UndefinedBehaviorSanitizer."""
+    plans = os.path.join(CSRC, "operator_plans.cpp")
+    deps = [HOST_CHECKS_SRC, plans, os.path.join(CSRC, "operators.cpp"),
+            os.path.join(os.path.dirname(HERE), "include", "eclat_hip.h")] + \
+        [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".hpp")]
+    if not force and os.path.exists(HOST_CHECKS) and os.path.getmtime(HOST_CHECKS) >= max(os.path.getmtime(p) for p in deps):
+        return HOST_CHECKS
+    _run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-fno-omit-frame-pointer",
+          "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__", "-I" + os.path.join(ROCM, "include"), HOST_CHECKS_SRC, plans,
+          "-static-libasan", "-static-libubsan", "-o", HOST_CHECKS])
+    return HOST_CHECKS
+
+
 if __name__ == "__main__":
     print(build(check="--check" in sys.argv))
     print(build_capi_client())

@@ -15,7 +15,9 @@ Buffer: shape, dtype, byte_len(), read_to_host() -> bytes,
 write_from_host(bytes), clone_buffer().  Kernel: execute(inputs, outputs).
 A backend may additionally provide compile_program(device, program_ast) for
 whole-program compilation (cross-kernel fusion); the executor uses it when
-present.
+present.  It may provide run_operator(device, name, attrs, inputs, outputs) for the operators
+that are no part of programs (`nn.token_logprobs`, `nn.distill_loss`, `nn.gated_scan`): inputs are
+(buffer, shape, dtype), outputs (shape, dtype), the result a buffer per output.
 """
 
 from __future__ import annotations
@@ -93,6 +95,12 @@ class EclatDevice:
 
     def compile_program(self, program):
         return self.backend.compile_program(self.device, program)
+
+    def supports_operators(self) -> bool:
+        return hasattr(self.backend, "run_operator")
+
+    def run_operator(self, name, attrs, inputs, outputs):
+        return self.backend.run_operator(self.device, name, attrs, inputs, outputs)
 
     def set_as_default(self) -> None:
         _tls.device = self

@@ -11,6 +11,11 @@ highest-numbered `bufN` is returned (`:389-447`).
 
 Backends that offer `compile_program` get the whole Program at once (buffer
 table attached) so they can fuse across kernels; results are identical.
+
+A graph with operator nodes (`graph.OperatorCall`; not in the reference) is run in stages: one
+program for what the calls that are ready read, then the calls, until only the roots are left.
+What a stage has computed is kept for the later ones; what only lies between is computed again
+where a later stage needs it.
 """
 
 from __future__ import annotations
@@ -21,9 +26,11 @@ from typing import Dict, List, Sequence
 from .ast import AstNode
 from .device import (DeviceError, compile_ast_with_cache, compile_program_with_cache,
                      get_default_device)
-from .graph import GraphNode, collect_inputs
+from .graph import GraphNode, collect_inputs, topological_sort
+from .graph import input as new_input
 from .lowerer import lower_graph
 from .optimize import optimize_program
+from .view import View
 
 
 class ExecutionError(Exception):
@@ -78,6 +85,91 @@ def _root_buffer_name(root: GraphNode, lowerer, available: Sequence[str], opt_ro
     return best[1] if best else None
 
 
+def _run_operators(roots: Sequence[GraphNode], input_buffers: Dict[int, object], fuse_program, constant_inputs):
+    """`execute_graph` of a graph with operator nodes."""
+    dev = get_default_device()
+    if not dev.supports_operators():
+        raise ExecutionError(f"Unsupported: backend '{dev.kind}' has no operators")
+    buffers, constants = dict(input_buffers), dict(constant_inputs or {})
+    owned = set()                                    # inputs of a stage that are this function's own buffers
+    values: Dict[object, GraphNode] = {}             # id(node) or (id(call), output) -> the input node that stands for it
+    keep = []
+
+    def key(n: GraphNode):
+        return (id(n.op.call), n.op.index) if n.op.kind == "operator" else id(n)
+
+    def put(n: GraphNode, buf) -> None:
+        stand_in = new_input([int(e.evaluate()) for e in n.shape()], n.dtype)
+        values[key(n)] = stand_in
+        buffers[id(stand_in)] = buf
+        owned.add(id(stand_in))
+        keep.append(n)
+
+    def rebuilt(nodes: Sequence[GraphNode]) -> List[GraphNode]:
+        """The graphs of `nodes` with what has been computed as inputs."""
+        memo: Dict[int, GraphNode] = {}
+        out = []
+        for root in nodes:
+            stack = [root]
+            while stack:
+                n = stack[-1]
+                if id(n) in memo:
+                    stack.pop()
+                elif key(n) in values:
+                    memo[id(n)] = values[key(n)]
+                else:
+                    todo = [s for s in n.src if id(s) not in memo]
+                    if todo:
+                        stack.extend(todo)
+                        continue
+                    src = [memo[id(s)] for s in n.src]
+                    memo[id(n)] = n if all(a is b for a, b in zip(src, n.src)) else n.with_new_sources(src)
+            out.append(memo[id(root)])
+        keep.append(memo)
+        return out
+
+    def evaluate(nodes: Sequence[GraphNode]) -> None:
+        """Dense buffers for `nodes`, whose graphs have no call left."""
+        todo = []
+        for n in nodes:
+            if key(n) not in values and n not in todo:
+                if n.is_external() and n.view == View.contiguous(n.shape()):
+                    values[key(n)] = n
+                else:
+                    todo.append(n)
+        if not todo:
+            return
+        graphs = [g if g.view == View.contiguous(g.shape()) and g.op.kind != "view" else g.contiguous() for g in rebuilt(todo)]
+        for n, buf in zip(todo, _execute(graphs, buffers, fuse_program, constants, owned)):
+            if buf is None:
+                raise ExecutionError("Internal: No output buffer returned from execution")
+            put(n, buf)
+
+    calls = []
+    for n in topological_sort(roots):
+        if n.op.kind == "operator" and all(n.op.call is not c for c in calls):
+            calls.append(n.op.call)
+    depth: Dict[int, int] = {}                       # calls behind one another in a node's graph
+
+    def depth_of(n: GraphNode) -> int:
+        for m in topological_sort([n]):
+            if id(m) not in depth:
+                depth[id(m)] = max([depth[id(s)] for s in m.src], default=0) + (1 if m.op.kind == "operator" else 0)
+        return depth[id(n)]
+    stages: Dict[int, list] = {}
+    for c in calls:
+        stages.setdefault(depth_of(c.nodes[0]), []).append(c)
+    for d in sorted(stages):
+        evaluate([s for c in stages[d] for s in c.src])
+        for c in stages[d]:
+            ins = [(buffers[id(values[key(s)])], [int(e.evaluate()) for e in s.shape()], s.dtype) for s in c.src]
+            for node, buf in zip(c.nodes, dev.run_operator(c.name, c.attrs, ins, c.outputs)):
+                put(node, buf)
+    rest = [r for r in roots if r.op.kind != "operator"]
+    results = iter(_execute(rebuilt(rest), buffers, fuse_program, constants, owned) if rest else [])
+    return [buffers[id(values[key(r)])] if r.op.kind == "operator" else next(results) for r in roots]
+
+
 def execute_graph(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
                   fuse_program: bool = None, constant_inputs: Dict[int, str] = None):
     """Returns one buffer per root (None where the reference finds none).
@@ -88,6 +180,14 @@ def execute_graph(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
         raise ExecutionError("NoDevice")
     if not roots:
         return []
+    if any(n.op.kind == "operator" for n in topological_sort(roots)):
+        return _run_operators(roots, input_buffers, fuse_program, constant_inputs)
+    return _execute(roots, input_buffers, fuse_program, constant_inputs, ())
+
+
+def _execute(roots, input_buffers, fuse_program, constant_inputs, owned):
+    """`execute_graph` of a graph without operator nodes; `owned`: inputs (by id) that need no copy."""
+    dev = get_default_device()
     program, lowerer, opt_roots = lower_graph(roots)
     # pipeline.optimize (executor.rs:169-176): ECLAT_OPT_LEVEL 0 leaves the program as lowered
     program = optimize_program(program)
@@ -98,7 +198,8 @@ def execute_graph(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
     for n in input_nodes:
         if id(n) not in input_buffers:
             raise ExecutionError(f"MissingInput: {lowerer.lookup_buffer_name(n)}")
-        buffer_map[lowerer.lookup_buffer_name(n) or ""] = input_buffers[id(n)].clone_buffer()
+        buf = input_buffers[id(n)]
+        buffer_map[lowerer.lookup_buffer_name(n) or ""] = buf if id(n) in owned else buf.clone_buffer()
 
     if fuse_program is None:
         fuse_program = os.environ.get("ECLAT_HIP_FUSE", "1") != "0"

@@ -80,8 +80,28 @@ def backward(output: GraphNode, params: Sequence[GraphNode], exact: bool = False
         memo[k] = r
         return r
 
-    for node in reversed(topological_sort([output])):
+    order = topological_sort([output])
+    # an operator's gradients are one call for all its outputs: made at the last of them, behind which
+    # only its sources follow
+    waiting: Dict[int, int] = {}
+    for node in order:
+        if node.op.kind == "operator":
+            waiting[id(node.op.call)] = waiting.get(id(node.op.call), 0) + 1
+    operator_grads: Dict[int, List[Optional[GraphNode]]] = {}
+    for node in reversed(order):
         g = ctx.get_grad(node)
+        if node.op.kind == "operator":
+            call = node.op.call
+            grads = operator_grads.setdefault(id(call), [None] * len(call.outputs))
+            if g is not None:
+                have = grads[node.op.index]
+                grads[node.op.index] = g if have is None else have + g
+            waiting[id(call)] -= 1
+            if waiting[id(call)] == 0 and call.vjp is not None and any(x is not None for x in grads):
+                for src, gi in zip(call.src, call.vjp(grads)):
+                    if gi is not None and needs_grad(src):
+                        ctx.accumulate_grad(src, gi)
+            continue
         if g is None or not node.src:
             continue
         for src, gi in zip(node.src, compute_vjp_exact(node, g) if exact else compute_vjp(node, g)):

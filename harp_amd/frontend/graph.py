@@ -61,8 +61,26 @@ def reduce_combine(op: str, acc: AstNode, val: AstNode) -> AstNode:
     raise ValueError(op)
 
 
+class OperatorCall:
+    """One call of a backend's hand-written operator on dense tensors (not in the reference).  Its
+    outputs are graph nodes of kind "operator" that share it; the executor runs the call between
+    programs (see `executor.py`).  `vjp(grads)` takes a gradient per output (None where there is none)
+    and returns one per source."""
+
+    __slots__ = ("name", "src", "attrs", "outputs", "vjp", "nodes")
+
+    def __init__(self, name: str, src, outputs, attrs=None, vjp=None):
+        self.name = name
+        self.src = list(src)
+        self.attrs = dict(attrs or {})
+        self.outputs = [(list(shape), dtype) for shape, dtype in outputs]
+        self.vjp = vjp
+        self.nodes = [GraphNode(self.src, View.contiguous(shape), GraphOp("operator", call=self, index=i), dtype)
+                      for i, (shape, dtype) in enumerate(self.outputs)]
+
+
 class GraphOp:
-    """kind: view | map_reduce | unfold | scatter | scan | matmul."""
+    """kind: view | map_reduce | unfold | scatter | scan | matmul | operator."""
 
     __slots__ = ("kind", "f")
 

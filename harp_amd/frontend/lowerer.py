@@ -238,6 +238,9 @@ class Lowerer:
             return self.lower_scan(node, out)
         if kind == "matmul":
             return self.lower_matmul(node, out)
+        if kind == "operator":
+            raise LoweringError(f"Unsupported operation: '{node.op.call.name}' runs between programs and is no part of one; "
+                                f"realize the tensors instead")
         raise LoweringError(f"Unsupported operation: {kind}")
 
     # -- helpers -----------------------------------------------------------------------

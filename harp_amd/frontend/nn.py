@@ -4,7 +4,8 @@ Host-side mirror of the reference's `crates/nn/src/functional/`:
 `activation.rs` (relu `:18-21`, leaky_relu `:34-39`, sigmoid `:50-57`, tanh `:70-76`,
 gelu `:88-99`, silu `:111-114`, elu `:127-135`, softmax `:148-160`, log_softmax `:174-187`,
 prelu `:201-210`), `linear.rs:27-56`, `conv.rs:26-92,113-187`, `pool.rs:117-162,172-213`,
-`attention.rs:22-96`, `loss.rs:32-65`.
+`attention.rs:22-96`, `loss.rs:32-65`; and the language-model operators that stand beside them as
+hand-written kernels (`token_logprobs`, `distill_loss`, `gated_scan`; not in the reference).
 The op trees are the reference's, including what follows from
 `Tensor::scale` ignoring its factor (so `tanh(x)` evaluates `sigmoid(x) - 1`) and from
 `Tensor::mean` being `sum`.  Functions whose meaning depends on such a factor take
@@ -13,8 +14,10 @@ The op trees are the reference's, including what follows from
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
+from . import graph as G
+from .ast import F32
 from .tensor import Tensor
 
 
@@ -199,3 +202,79 @@ def cross_entropy_loss(logits: Tensor, one_hot: Tensor, exact: bool = False) -> 
     n = logits.shape()[0]
     total = (one_hot * log_softmax(logits, 1)).sum(1).sum(0)
     return total.scale_exact(-1.0 / n) if exact else total.scale(-1.0 / n)
+
+
+# ---- language-model operators (harp_amd/operators.py) ---------------------------------------------------
+#
+# Nodes of the graph like any other, with gradients in both modes, but run between programs: a step
+# with one of them takes several programs, and `CompiledStep`, which is one, does not hold them.
+
+
+def _f32(name: str, *tensors: Tensor) -> None:
+    for t in tensors:
+        if t.dtype() != F32:
+            raise ValueError(f"{name}: f32 tensors, got {t.dtype()}")
+
+
+def _integers(name: str, t: Tensor) -> None:
+    if t.dtype().name not in ("i32", "i64"):
+        raise ValueError(f"{name}: ids are i32 or i64, got {t.dtype()}")
+
+
+def token_logprobs(logits: Tensor, targets: Tensor, scale: float = 1.0, ignore_index: int = -1) -> Tuple[Tensor, Tensor]:
+    """The log probability of the token `targets` [N] (i32 or i64; `ignore_index`: none, 0) of each row of
+    `logits` [N,V] under softmax(scale * logits), and the rows' entropies: two tensors [N].  The negated
+    sum of the first over a batch is `cross_entropy_loss` without a one-hot tensor."""
+    _f32("token_logprobs", logits)
+    _integers("token_logprobs", targets)
+    if len(logits.shape()) != 2 or targets.shape() != logits.shape()[:1]:
+        raise ValueError(f"token_logprobs: logits [N,V] and targets [N], got {logits.shape()} and {targets.shape()}")
+    n, v = logits.shape()
+    attrs = {"scale": float(scale), "ignore_index": int(ignore_index)}
+
+    def vjp(grads):
+        g, e, _ = grads
+        src = [logits.graph, targets.graph, call.nodes[2], call.nodes[1]] + [x for x in (g, e) if x is not None]
+        back = G.OperatorCall("token_logprobs_backward", src, [([n, v], F32)], {**attrs, "logp": g is not None, "entropy": e is not None})
+        return [back.nodes[0], None]
+    call = G.OperatorCall("token_logprobs", [logits.graph, targets.graph], [([n], F32), ([n], F32), ([n, 2], F32)], attrs, vjp)
+    return Tensor(call.nodes[0]), Tensor(call.nodes[1])
+
+
+def distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_ids: Tensor, temperature: float = 1.0) -> Tensor:
+    """temperature^2 KL(teacher || student) of each row [N]: the student's softmax(logits / temperature) over
+    [N,V], the teacher's over the tokens `teacher_ids` [N,K] (negative: no entry) with `teacher_logits` [N,K].  The
+    gradient is that of the student's logits; the teacher is a constant."""
+    _f32("distill_loss", logits, teacher_logits)
+    _integers("distill_loss", teacher_ids)
+    if len(logits.shape()) != 2 or len(teacher_logits.shape()) != 2 or teacher_logits.shape() != teacher_ids.shape() or \
+            teacher_logits.shape()[0] != logits.shape()[0]:
+        raise ValueError(f"distill_loss: logits [N,V], teacher's logits and ids [N,K], got {logits.shape()}, {teacher_logits.shape()}, {teacher_ids.shape()}")
+    n, v = logits.shape()
+    attrs = {"temperature": float(temperature)}
+
+    def vjp(grads):
+        if grads[0] is None:
+            return [None, None, None]
+        back = G.OperatorCall("distill_loss_backward", call.src + [call.nodes[1], grads[0]], [([n, v], F32)], attrs)
+        return [back.nodes[0], None, None]
+    call = G.OperatorCall("distill_loss", [logits.graph, teacher_logits.graph, teacher_ids.graph], [([n], F32), ([n, 2], F32)], attrs, vjp)
+    return Tensor(call.nodes[0])
+
+
+def gated_scan(gate: Tensor, x: Tensor, state: Optional[Tensor] = None, log_gate: bool = False) -> Tensor:
+    """The gated linear recurrence h_t = a_t h_(t-1) + x_t along axis 1 of [B,T,D], a = gate or exp(gate), h_(-1) =
+    `state` [B,D] or 0 (with gates of one a running sum).  Its last step is the next call's `state`."""
+    _f32("gated_scan", gate, x, *([state] if state is not None else []))
+    if len(gate.shape()) != 3 or gate.shape() != x.shape() or (state is not None and state.shape() != [gate.shape()[0], gate.shape()[2]]):
+        raise ValueError(f"gated_scan: gate and x [B,T,D], state [B,D], got {gate.shape()}, {x.shape()}" + (f", {state.shape()}" if state is not None else ""))
+    b, t, d = gate.shape()
+    src = [gate.graph, x.graph] + ([state.graph] if state is not None else [])
+    attrs = {"log_gate": bool(log_gate)}
+
+    def vjp(grads):
+        outs = [([b, t, d], F32), ([b, t, d], F32)] + ([([b, d], F32)] if state is not None else [])
+        back = G.OperatorCall("gated_scan_backward", [gate.graph, call.nodes[0], grads[0]] + src[2:], outs, attrs)
+        return back.nodes
+    call = G.OperatorCall("gated_scan", src, [([b, t, d], F32)], attrs, vjp)
+    return Tensor(call.nodes[0])

@@ -85,47 +85,53 @@ def _code(dtype, name):
 
 def _array(device, x, name, ndim, want=None):
     """(shape, element type, fields of an eh_array) of an array; `want`: the shape it has to have."""
-    if isinstance(x, HipBuffer) or isinstance(x, View):
-        buf = x if isinstance(x, HipBuffer) else x.buffer
-        if buf.device is not device:
-            raise ValueError(f"{name}: lives on another device handle")
-        if x.dtype is None:
-            raise TypeError(f"{name}: the buffer has no element type")
-        shape = tuple(x.shape)
-        strides = _dense(shape) if buf is x else x.strides
-        address = None
-    else:
-        try:
-            address, shape, strides, index = x.data_ptr(), x.shape, x.stride(), x.get_device()
-        except AttributeError:
-            raise TypeError(f"{name}: a {type(x).__name__} is no array on the device") from None
-        if index != device.index:
-            raise ValueError(f"{name}: lives on " + ("the host" if index < 0 else f"GPU {index}") + f", the handle is of GPU {device.index}")
+    try:
+        address, shape, strides = x.data_ptr(), x.shape, x.stride()
+        index, dtype = x.get_device(), x.dtype
+    except AttributeError:
+        return _buffer_array(device, x, name, ndim, want)
+    if index != device.index:
+        raise ValueError(f"{name}: lives on " + ("the host" if index < 0 else f"GPU {index}") + f", the handle is of GPU {device.index}")
+    code = _known.get(dtype)
+    if code is None:
+        code = _code(dtype, name)
+    s0, s1, last = _layout(name, shape, strides, ndim, want)
+    if last <= 0:                                    # an empty tensor has no address
+        return shape, code, (0, 16, 0, s0, s1, code)
+    return shape, code, (0, address, last * _ITEM[code], s0, s1, code)
+
+
+def _buffer_array(device, x, name, ndim, want):
+    buf = x.buffer if isinstance(x, View) else x
+    if not isinstance(buf, HipBuffer):
+        raise TypeError(f"{name}: a {type(x).__name__} is no array on the device")
+    if buf.device is not device:
+        raise ValueError(f"{name}: lives on another device handle")
+    if x.dtype is None:
+        raise TypeError(f"{name}: the buffer has no element type")
     code = _known.get(x.dtype)
     if code is None:
         code = _code(x.dtype, name)
-    if len(shape) != ndim or (want is not None and tuple(shape) != want):
-        raise ValueError(f"{name}: shape {tuple(shape)}, expected " + (f"{ndim} axes" if want is None else str(want)))
+    shape = tuple(x.shape)
+    strides, offset = (_dense(shape), 0) if buf is x else (x.strides, x.offset)
+    if offset < 0:
+        raise ValueError(f"{name}: starts before its buffer")
+    s0, s1, _ = _layout(name, shape, strides, ndim, want)
+    return shape, code, (buf._h.value, offset, 0, s0, s1, code)
+
+
+def _layout(name, shape, strides, ndim, want):
+    """The outer strides, and how many elements lie between the first and the last."""
+    if want is not None and shape != want or len(shape) != ndim:
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected " + (f"{ndim} axes" if want is None else str(tuple(want))))
+    n = shape[-1]
+    if n > 1 and strides[-1] != 1:
+        raise ValueError(f"{name}: " + ("has to be contiguous" if ndim == 1 else "the last axis has to be contiguous"))
     if ndim == 1:
-        s0, s1, n = strides[0], 0, shape[0]
-        last = (n - 1) * s0 + 1 if n else 0
-        if s0 != 1 and n > 1:
-            raise ValueError(f"{name}: has to be contiguous")
-    elif ndim == 2:
-        s0, s1, n = strides[0], 0, shape[1]
-        last = (shape[0] - 1) * s0 + n if n and shape[0] else 0
-        if strides[1] != 1 and n > 1:
-            raise ValueError(f"{name}: the last axis has to be contiguous")
-    else:
-        s0, s1, n = strides[0], strides[1], shape[2]
-        last = (shape[0] - 1) * s0 + (shape[1] - 1) * s1 + n if n and shape[0] and shape[1] else 0
-        if strides[2] != 1 and n > 1:
-            raise ValueError(f"{name}: the last axis has to be contiguous")
-    if address is None:
-        return shape, code, (buf._h.value, 0 if buf is x else x.offset, 0, s0, s1, code)
-    if not last:                                     # an empty tensor has no address
-        return shape, code, (0, 16, 0, s0, s1, code)
-    return shape, code, (0, address, last * _ITEM[code], s0, s1, code)
+        return 1, 0, n
+    if ndim == 2:
+        return strides[0], 0, (shape[0] - 1) * strides[0] + n if n and shape[0] else 0
+    return strides[0], strides[1], (shape[0] - 1) * strides[0] + (shape[1] - 1) * strides[1] + n if n and shape[0] and shape[1] else 0
 
 
 def _small(device, x, name, want, code):
@@ -311,3 +317,33 @@ def gated_scan_backward_workspace(device: HipDevice, gate) -> int:
     """Bytes `gated_scan_backward` works in besides its arrays; needed as `workspace` under stream capture."""
     shape, _, g = _array(device, gate, "gate", 3)
     return _bytes_needed(lib.eh_gated_scan_backward_workspace, device, _SCAN_GRAD.pack(*shape, 0, *g, *(9 * _NONE)))
+
+
+# ---- the front end's calls ----------------------------------------------------------------------------
+
+
+def run(device: HipDevice, name: str, attrs: dict, inputs, outputs):
+    """An operator node of a graph: `inputs` (buffer, shape, dtype), dense; `outputs` (shape, dtype).  Returns the
+    outputs' buffers."""
+    ins = [View(b, shape, dtype) for b, shape, dtype in inputs]
+    outs = [HipBuffer(device, shape, dtype) for shape, dtype in outputs]
+    if name == "token_logprobs":
+        token_logprobs(device, *ins, out=Logprobs(*outs, None, None), **attrs)
+    elif name == "token_logprobs_backward":
+        logits, targets, norm, entropy, *grads = ins
+        g = grads.pop(0) if attrs["logp"] else None
+        e = grads.pop(0) if attrs["entropy"] else None
+        token_logprobs_backward(device, logits, targets, norm, entropy, g, e, scale=attrs["scale"],
+                                ignore_index=attrs["ignore_index"], out=outs[0])
+    elif name == "distill_loss":
+        distill_loss(device, *ins, out=Distilled(*outs, None), **attrs)
+    elif name == "distill_loss_backward":
+        distill_loss_backward(device, *ins, out=outs[0], **attrs)
+    elif name == "gated_scan":
+        gated_scan(device, *ins[:2], state=ins[2] if len(ins) > 2 else None, out=outs[0], **attrs)
+    elif name == "gated_scan_backward":
+        gated_scan_backward(device, *ins[:3], state=ins[3] if len(ins) > 3 else None,
+                            out=ScanGrads(*outs, *[None] * (3 - len(outs))), **attrs)
+    else:
+        raise ValueError(f"no operator '{name}'")
+    return outs

@@ -152,5 +152,9 @@ class CBackend:
     def allocate_buffer(self, device, shape, dtype) -> CBuffer:
         return CBuffer(shape, dtype)
 
+    def run_operator(self, device, name, attrs, inputs, outputs):
+        from . import operators
+        return operators.run(CBuffer, name, attrs, inputs, outputs)
+
     def compile_ast(self, device, program, signature=None) -> CKernel:
         return compile_program_text(program.to_sexpr(), openmp=self.openmp, gcc_args=self.gcc_args)
