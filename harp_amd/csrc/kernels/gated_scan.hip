@@ -41,10 +41,18 @@ __device__ inline unsigned int word_of(float x) {
   return b == kEmpty ? 0x7fc00000u : b;
 }
 
-// Up to N channels of one step; those behind the row's end are 0.
-template <int DT> __device__ inline u32x4 load_some(const typename Elem<DT>::T* p, int n) {
+// The last n < N channels of a row of `width`; what lies behind them is 0.  A row of at least a vector
+// is read by the vector that ends with it.
+template <int DT> __device__ inline u32x4 load_last(const typename Elem<DT>::T* p, int n, int width) {
   constexpr int N = Elem<DT>::N;
   u32x4 v = {0, 0, 0, 0};
+  if (width >= N) {
+    v = load16(p - (N - n));
+    const uint64_t lo = v[0] | static_cast<uint64_t>(v[1]) << 32, hi = v[2] | static_cast<uint64_t>(v[3]) << 32;
+    const int bits = (N - n) * (128 / N);                  // 0 < bits < 128
+    const uint64_t l = bits < 64 ? lo >> bits | hi << 1 << (63 - bits) : hi >> (bits - 64), h = bits < 64 ? hi >> bits : 0;
+    return u32x4{static_cast<uint32_t>(l), static_cast<uint32_t>(l >> 32), static_cast<uint32_t>(h), static_cast<uint32_t>(h >> 32)};
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     if (j >= n) break;
@@ -70,28 +78,39 @@ template <int DT, bool FAR> struct PieceRows {
 };
 
 // kSteps rows from `row` on, each held inside [0, most].
-template <int DT, bool FAR> __device__ inline void load_steps(const PieceRows<DT, FAR>& s, int row, int most, uint32_t cb, int nc, u32x4* v) {
+template <int DT, bool FAR> __device__ inline void load_steps(const PieceRows<DT, FAR>& s, int row, int most, uint32_t cb, int nc, int width, u32x4* v) {
   if (nc >= Elem<DT>::N) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) v[i] = load16(s.at(max(min(row + i, most), 0), cb));
   } else {
-#pragma unroll 1
-    for (int i = 0; i < kSteps; ++i) {
-      const u32x4 x = load_some<DT>(s.at(max(min(row + i, most), 0), cb), nc);
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) v[k] = k == i ? x : v[k];
-    }
+    for (int i = 0; i < kSteps; ++i) v[i] = load_last<DT>(s.at(max(min(row + i, most), 0), cb), nc, width);
   }
 }
 template <int DT> __device__ inline void store_channels(typename Elem<DT>::T* p, int n, const float* z) {
   constexpr int N = Elem<DT>::N;
+  typedef uint32_t __attribute__((aligned(2))) any32;
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef u32x2 __attribute__((aligned(2))) any64;
   if (n >= N) {
     store16(p, Elem<DT>::pack(z));
     return;
   }
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (j < n) p[j] = Elem<DT>::put(z[j]);
+  const u32x4 v = Elem<DT>::pack(z);
+  // eight bytes, four, two: whichever n has
+  constexpr int half = N / 2;
+  uint32_t a = v[0], b = v[1];
+  if (n & half) {
+    *reinterpret_cast<any64*>(p) = u32x2{a, b};
+    p += half, a = v[2], b = v[3];
+  }
+  if (n & (half / 2)) {
+    *reinterpret_cast<any32*>(p) = a;
+    p += half / 2, a = b;
+  }
+  if constexpr (N == 8) {
+    if (n & 1) *p = static_cast<uint16_t>(a);
+  }
 }
 
 // The gates and the added values of a step; behind a sequence's end the step changes nothing.
@@ -185,8 +204,8 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
 
   u32x4 vg[kSteps] = {}, vx[kSteps] = {};
   if (n > 0 && nc > 0) {
-    load_steps<DT, FAR>({a.gate, b, k * RUN, tile}, row, rows - 1, cb, nc, vg);
-    load_steps<DT, FAR>({BACK ? a.out : a.x, b, k * RUN, tile}, row, rows - 1, cb, nc, vx);
+    load_steps<DT, FAR>({a.gate, b, k * RUN, tile}, row, rows - 1, cb, nc, a.width, vg);
+    load_steps<DT, FAR>({BACK ? a.out : a.x, b, k * RUN, tile}, row, rows - 1, cb, nc, a.width, vx);
   }
   float A[N], B[N];
 #pragma unroll
@@ -308,7 +327,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     u32x4 vh[kSteps];
     // h of the step before each: the rows from the piece before's last on; the first step of all has the state
     const int first = k > 0 ? 1 : 0;
-    if (n > 0) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, vh);
+    if (n > 0) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, a.width, vh);
 #pragma unroll
     for (int i = kSteps - 1; i >= 0; --i) {
       if (row + i >= rows) continue;                                       // h stays what came from behind
