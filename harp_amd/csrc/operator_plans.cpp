@@ -12,20 +12,28 @@ namespace eh {
 // and 1021 x 50257 f16 with 5: 256 threads 27, 512 34 (its workgroups are all on the device at once, more
 // threads only lengthen the selection).  Segments only pay where a row is long and there are few:
 // 1 x 150000 f32 11.7 against 15.6 with one workgroup of 1024, 64 x 150000 bf16 16.6 against 17.8.
-RowSplit split_rows(int64_t rows, int vocab, int dtype, int compute_units) {
+// Without alternatives a row goes to the registers of the smallest workgroup that holds it, us against the kernel
+// that streams, 16384 rows: x 500 bf16 8.1 : 10.2, 2000 14 : 22, 6000 33 : 37, 8000 39 : 50, 12000 78 : 77, 16000
+// 93 : 101, f32 x 4000 37 : 43; with 1024 threads only few rows (8192 x 32000 bf16 107 : 97, 8 x 32000 7.3 : 7.5).
+RowSplit split_rows(int64_t rows, int vocab, int dtype, bool top, int compute_units) {
   const int vec = 16 / static_cast<int>(elem_size(dtype));
-  const int64_t items = (vocab + vec - 1) / vec;
+  const int64_t items = (vocab + vec - 1) / vec, held = items + 1;       // one more where a row starts between two
   if (items > 32768 && rows * 4 <= compute_units) {
     // 32 KB a segment at least, four vectors for each of 512 threads
     const int64_t want = (2 * static_cast<int64_t>(compute_units) + rows - 1) / rows;
     const int64_t segs = std::min<int64_t>(want, items / 2048);
     const int64_t seg = (items + segs - 1) / segs * vec;
-    return {512, static_cast<int>((vocab + seg - 1) / seg), static_cast<int>(seg)};
+    return {512, 0, static_cast<int>((vocab + seg - 1) / seg), static_cast<int>(seg)};
   }
-  if (rows <= compute_units) return {items <= 256 ? 64 : items <= 512 ? 128 : items <= 1024 ? 256 : items <= 2048 ? 512 : 1024, 1, vocab};
-  if (items <= 512) return {64, 1, vocab};
-  if (items <= 2048) return {128, 1, vocab};
-  return {items > 4096 && rows >= 8 * static_cast<int64_t>(compute_units) ? 512 : 256, 1, vocab};
+  if (!top) {
+    for (int threads = 64; threads <= (rows <= compute_units ? 1024 : 512); threads *= 2)
+      for (int n = 1; n <= kScoreHeld; ++n)
+        if (held_form(threads, n) && held <= n * threads) return {threads, n, 1, vocab};
+  }
+  if (rows <= compute_units) return {items <= 256 ? 64 : items <= 512 ? 128 : items <= 1024 ? 256 : items <= 2048 ? 512 : 1024, 0, 1, vocab};
+  if (items <= 512) return {64, 0, 1, vocab};
+  if (items <= 2048) return {128, 0, 1, vocab};
+  return {items > 4096 && rows >= 8 * static_cast<int64_t>(compute_units) ? 512 : 256, 0, 1, vocab};
 }
 
 size_t split_workspace(const RowSplit& s, int64_t rows, int top) {

@@ -242,11 +242,10 @@ void check_sequences(int64_t batch, int64_t time, int64_t width) {
 
 int units(const HipDevice& d) { return std::max(d.profile().compute_units, 1); }
 
-// Float logits may be given with an element type of their own; nothing else decides the split.
-RowSplit split_of(const HipDevice& d, int64_t rows, int64_t vocab, const eh_array& logits) {
+RowSplit split_of(const HipDevice& d, int64_t rows, int64_t vocab, const eh_array& logits, bool top) {
   if (!is_float(logits.dtype)) throw Error("logits: has to be f32, bf16 or f16");
-  if (rows == 0) return {64, 1, static_cast<int>(vocab)};
-  return split_rows(rows, static_cast<int>(vocab), static_cast<int>(logits.dtype), units(d));
+  if (rows == 0) return {64, 0, 1, static_cast<int>(vocab)};
+  return split_rows(rows, static_cast<int>(vocab), static_cast<int>(logits.dtype), top, units(d));
 }
 
 void check_top(const eh_token_logprobs_args* a) {
@@ -285,7 +284,7 @@ int eh_token_logprobs_workspace(eh_device* dev, const eh_token_logprobs_args* ar
   return guard([&] {
     check_rows(args->rows, args->vocab);
     check_top(args);
-    *bytes = split_workspace(split_of(dev->dev, args->rows, args->vocab, args->logits), args->rows, static_cast<int>(args->top));
+    *bytes = split_workspace(split_of(dev->dev, args->rows, args->vocab, args->logits, args->top > 0), args->rows, static_cast<int>(args->top));
   });
 }
 
@@ -312,7 +311,7 @@ int eh_token_logprobs(eh_device* dev, const eh_token_logprobs_args* args, int sy
       s.top_logp = arrays.small<float>("top_logp", a.top_logp, a.rows, a.top, EH_F32, true, true);
       s.top_ids = arrays.small<int>("top_ids", a.top_ids, a.rows, a.top, EH_I32, true, true);
     }
-    s.split = split_of(*d, a.rows, a.vocab, a.logits);
+    s.split = split_of(*d, a.rows, a.vocab, a.logits, a.top > 0);
     Workspace ws(d, arrays, a.workspace, split_workspace(s.split, a.rows, s.top));
     s.workspace = ws.at();
     arrays.settle();
@@ -353,7 +352,7 @@ int eh_distill_loss_workspace(eh_device* dev, const eh_distill_loss_args* args, 
   REQUIRE(dev && args && bytes, "device, args or bytes is NULL");
   return guard([&] {
     check_rows(args->rows, args->vocab);
-    *bytes = split_workspace(split_of(dev->dev, args->rows, args->vocab, args->logits), args->rows, 0);
+    *bytes = split_workspace(split_of(dev->dev, args->rows, args->vocab, args->logits, false), args->rows, 0);
   });
 }
 
@@ -380,7 +379,7 @@ static void distill(eh_device* dev, const eh_distill_loss_args& a, bool backward
     s.grad = arrays.floats("grad", a.grad, a.rows, 1, a.vocab, a.logits.dtype, true);
     s.grad_stride = a.grad.stride[0];
   }
-  s.split = split_of(*d, a.rows, a.vocab, a.logits);
+  s.split = split_of(*d, a.rows, a.vocab, a.logits, false);
   s.held = hold_rows(a.rows, s.in.vocab, s.in.dtype, units(*d));
   const eh_array none{};
   Workspace ws(d, arrays, backward ? none : a.workspace, backward ? 0 : split_workspace(s.split, a.rows, 0));

@@ -33,12 +33,15 @@ struct TokenIds {
 
 // How a pass over rows that reads each once goes to workgroups: a row to one of `threads` threads, or
 // `segs` segments of `seg` elements with a second launch that joins them.
+constexpr int kScoreHeld = 4;        // most items (16 bytes) of a thread in a row that is held in registers
+constexpr bool held_form(int threads, int items) { return items == kScoreHeld || threads == 64 || (items == 3 && threads < 1024); }
 struct RowSplit {
   int threads;
+  int held;                // items a thread of a row held in registers (held_form), or 0
   int segs;
   int seg;
 };
-RowSplit split_rows(int64_t rows, int vocab, int dtype, int compute_units);
+RowSplit split_rows(int64_t rows, int vocab, int dtype, bool top, int compute_units);
 // What a segment leaves for the join (its best keys, 8 bytes each, follow).
 struct RowPartial {
   float largest, s, t, pad;

@@ -405,11 +405,14 @@ static void plans() {
     const int dtype = i % 3, vec = 16 / static_cast<int>(elem_size(dtype));
     const int64_t rows = next(1, 1 << 24);
     const int vocab = static_cast<int>(next(1, 1 << 30));
-    const RowSplit r = split_rows(rows, vocab, dtype, 256);
+    const bool top = i % 5 == 0;
+    const RowSplit r = split_rows(rows, vocab, dtype, top, 256);
     bool ok = (r.threads == 64 || r.threads == 128 || r.threads == 256 || r.threads == 512 || r.threads == 1024) && r.segs >= 1;
     // the last segment is not empty, the others are whole, a launch's workgroups are countable
     ok = ok && static_cast<int64_t>(r.segs - 1) * r.seg < vocab && static_cast<int64_t>(r.segs) * r.seg >= vocab;
     ok = ok && (r.segs == 1 || (r.seg % vec == 0 && r.threads == 512)) && rows * r.segs < (int64_t{1} << 31);
+    // a row held in registers fits them wherever it starts
+    ok = ok && (!r.held || (!top && r.segs == 1 && held_form(r.threads, r.held) && static_cast<int64_t>(r.threads) * r.held * vec >= static_cast<int64_t>(vocab) + vec - 1));
     const RowHeld h = hold_rows(rows, vocab, dtype, 256);
     ok = ok && (h.vectors == 0 || static_cast<int64_t>(h.threads) * h.vectors >= vocab / vec);
     ok = ok && (h.vectors == 0 || (h.vectors == 4 && (h.threads == 64 || h.threads == 256 || h.threads == 1024)) ||
