@@ -42,16 +42,21 @@ __device__ inline unsigned int word_of(float x) {
 }
 
 // The last n < N channels of a row of `width`; what lies behind them is 0.  A row of at least a vector
-// is read by the vector that ends with it.
+// is read by the vector that ends with it, moved down by whole words and then by half a one: 32 bits at a time,
+// since a 64-bit shift whose amount is in the last register that a kernel has was seen to take v0's
+// value for it now and then (the gradient of 13 x 1999 x 717 f16 had about 1000 wrong channels).
 template <int DT> __device__ inline u32x4 load_last(const typename Elem<DT>::T* p, int n, int width) {
   constexpr int N = Elem<DT>::N;
   u32x4 v = {0, 0, 0, 0};
   if (width >= N) {
-    v = load16(p - (N - n));
-    const uint64_t lo = v[0] | static_cast<uint64_t>(v[1]) << 32, hi = v[2] | static_cast<uint64_t>(v[3]) << 32;
-    const int bits = (N - n) * (128 / N);                  // 0 < bits < 128
-    const uint64_t l = bits < 64 ? lo >> bits | hi << 1 << (63 - bits) : hi >> (bits - 64), h = bits < 64 ? hi >> bits : 0;
-    return u32x4{static_cast<uint32_t>(l), static_cast<uint32_t>(l >> 32), static_cast<uint32_t>(h), static_cast<uint32_t>(h >> 32)};
+    const int down = N - n, words = N == 4 ? down : down / 2;
+    v = load16(p - down);
+    if (words & 2) v = u32x4{v[2], v[3], 0, 0};
+    if (words & 1) v = u32x4{v[1], v[2], v[3], 0};
+    if (N == 8 && (down & 1)) {
+      v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+    }
+    return v;
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) {

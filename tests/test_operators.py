@@ -391,6 +391,15 @@ def test_scan_layouts(dev, ops, layout, dtype):
     check_scan(dev, ops, 2, 513, 41, dtype, log_gate=False, layout=layout)
 
 
+@pytest.mark.parametrize("log_gate", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scan_last_channels(dev, ops, dtype, log_gate):
+    """Rows that end inside a vector, in many workgroups at once: with every count of channels in the last one."""
+    check_scan(dev, ops, 6, 1030, 717, dtype, log_gate, lengths=[1030, 1, 513, 1029, 700, 1030])
+    for width in (65, 74, 83, 92, 102, 111):
+        check_scan(dev, ops, 3, 530, width, dtype, log_gate)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_scan_lengths(dev, ops, dtype):
     """Sequences of no steps, one, all, and lengths outside the array; NaN behind them stays there."""

@@ -1,6 +1,8 @@
 """The language-model operators without a GPU: the C entry points' checks and plans (operators_host.cpp, under
 AddressSanitizer and UndefinedBehaviorSanitizer), and what the Python side refuses before it calls them."""
 
+import os
+import re
 import subprocess
 
 import pytest
@@ -14,6 +16,21 @@ def test_entry_points_and_plans():
     r = subprocess.run([build.build_operator_checks()], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-3000:]
     assert r.stdout.strip().endswith(" 0 failed")
+
+
+@pytest.mark.parametrize("source", ["gated_scan", "token_rows"])
+def test_no_shift_by_the_last_register(source, tmp_path):
+    """A 64-bit shift whose amount is in the last register of a kernel's allocation was seen to take another
+    register's value for it: no kernel has one."""
+    out = str(tmp_path / "code.s")
+    subprocess.run([os.path.join(build.ROCM, "bin", "hipcc"), "-std=c++17", *build.DEVICE_FLAGS, "--offload-device-only", "-S",
+                    os.path.join(build.CSRC, "kernels", source + ".hip"), "-o", out], check=True, capture_output=True, timeout=300)
+    with open(out) as f:
+        kernels = re.findall(r"\n(_Z\S+):(.*?)\.amdhsa_next_free_vgpr (\d+)", f.read(), re.S)
+    assert kernels
+    for name, code, registers in kernels:
+        last = (int(registers) + 7) // 8 * 8 - 1
+        assert not re.search(r"v_(lshlrev|lshrrev|ashrrev)_[bi]64\S* v\[\d+:\d+\], v%d," % last, code), name
 
 
 class Tensor:
