@@ -41,23 +41,24 @@ __device__ inline unsigned int word_of(float x) {
   return b == kEmpty ? 0x7fc00000u : b;
 }
 
-// The last n < N channels of a row of `width`; what lies behind them is 0.  A row of at least a vector
-// is read by the vector that ends with it, moved down by whole words and then by half a one: 32 bits at a time,
-// since a 64-bit shift whose amount is in the last register that a kernel has was seen to take v0's
-// value for it now and then (the gradient of 13 x 1999 x 717 f16 had about 1000 wrong channels).
-template <int DT> __device__ inline u32x4 load_last(const typename Elem<DT>::T* p, int n, int width) {
+// A row of at least a vector is read by the vector that ends with it, which `down` channels are moved out of: by
+// whole words, then by half a one.  32 bits at a time, since a 64-bit shift whose amount is in the last
+// register that a kernel has was seen to take v0's value for it now and then (the gradient of 13 x 1999 x 717
+// f16 had about 1000 wrong channels).  What comes in is 0.
+template <int DT> __device__ inline u32x4 move_down(u32x4 v, int down) {
+  constexpr int N = Elem<DT>::N;
+  const int words = N == 4 ? down : down / 2;
+  if (words & 2) v = u32x4{v[2], v[3], 0, 0};
+  if (words & 1) v = u32x4{v[1], v[2], v[3], 0};
+  if (N == 8 && (down & 1)) {
+    v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+  }
+  return v;
+}
+// The n < N channels of a row that has no more; what lies behind them is 0.
+template <int DT> __device__ inline u32x4 load_few(const typename Elem<DT>::T* p, int n) {
   constexpr int N = Elem<DT>::N;
   u32x4 v = {0, 0, 0, 0};
-  if (width >= N) {
-    const int down = N - n, words = N == 4 ? down : down / 2;
-    v = load16(p - down);
-    if (words & 2) v = u32x4{v[2], v[3], 0, 0};
-    if (words & 1) v = u32x4{v[1], v[2], v[3], 0};
-    if (N == 8 && (down & 1)) {
-      v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
-    }
-    return v;
-  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     if (j >= n) break;
@@ -82,14 +83,22 @@ template <int DT, bool FAR> struct PieceRows {
   }
 };
 
-// kSteps rows from `row` on, each held inside [0, most].
-template <int DT, bool FAR> __device__ inline void load_steps(const PieceRows<DT, FAR>& s, int row, int most, uint32_t cb, int nc, int width, u32x4* v) {
-  if (nc >= Elem<DT>::N) {
+// kSteps rows from `row` on, each held inside [0, most].  All loads go out together, those of a row's last
+// channels too (32 x 512 x 717 f16 16 us and its gradient 23; with those one after the other 21 and 31).
+template <int DT, bool FAR> __device__ inline void load_steps(PieceRows<DT, FAR> s, int row, int most, uint32_t cb, int nc, int width, u32x4* v) {
+  constexpr int N = Elem<DT>::N;
+  if (width >= N) {
+    s.base -= 16;                                           // so that offsets stay above 0
+    cb += 16 - static_cast<uint32_t>(max(N - nc, 0) * sizeof(typename Elem<DT>::T));
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) v[i] = load16(s.at(max(min(row + i, most), 0), cb));
+    if (nc < N) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) v[i] = move_down<DT>(v[i], N - width % N);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) v[i] = load_last<DT>(s.at(max(min(row + i, most), 0), cb), nc, width);
+    for (int i = 0; i < kSteps; ++i) v[i] = load_few<DT>(s.at(max(min(row + i, most), 0), cb), nc);
   }
 }
 template <int DT> __device__ inline void store_channels(typename Elem<DT>::T* p, int n, const float* z) {
@@ -175,6 +184,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
       turn[0] = -1;
       for (int i = 0; i < classes; ++i) {
         const Class c(columns, classes, (blockIdx.x + i) % classes);
+        if (c.columns == 0) continue;
         const unsigned int t = atomicAdd(board.tickets + c.number * kTicketStride, 1u) + 1u;      // the words start at all ones
         if (t < c.columns * pieces) {
           turn[0] = c.first + t % c.columns;
