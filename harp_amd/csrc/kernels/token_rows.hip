@@ -428,11 +428,12 @@ template <int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS)
 
 // dz_i = c [ g ([i = t] - p_i) - e p_i (log p_i + H) ] with g, e the gradients of log p_t and H: one
 // pass, a vector for each thread.  Workgroups of 4 KB keep what is on the way in memory order:
-// 8192 x 65536 bf16 in 337 us (6.4 TB/s); 362 us with two vectors a thread, 415 us with a row for a workgroup.
-template <int DT, bool ENT> __global__ __launch_bounds__(256) void score_grad_rows(ScoreGradArgs a, int spans) {
+// 8192 x 65536 bf16 in 384 us (5.6 TB/s; a copy of as much reaches 5.0); more vectors a thread, or a row for a
+// workgroup, were 7 and 20% slower.
+template <int DT, bool ENT> __global__ __launch_bounds__(256) void score_grad_rows(ScoreGradArgs a, int spans, int64_t row0) {
   constexpr int N = Elem<DT>::N;
   typedef typename Elem<DT>::T T;
-  const int64_t row = blockIdx.x / spans;
+  const int64_t row = row0 + blockIdx.x / spans;
   const int at = (static_cast<int>(blockIdx.x % spans) * 256 + static_cast<int>(threadIdx.x)) * N, n = a.in.vocab - at;
   if (n <= 0) return;
   const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride + at;
@@ -595,7 +596,7 @@ __device__ inline void write_named(const Teacher& t, const Gradient& g, typename
 // A row to a workgroup, in its registers (THREADS * NV vectors) from one reading: the loss and the
 // gradient.  What concerns the teacher is found while the logits arrive.  Bound by memory, with one
 // row of 250 KB on a compute unit by the waits between its reading and its writing too: 8192 x 128000
-// bf16 in 820 us (5.1 TB/s).  Read a second time instead: 1280 us with four times as many rows on the
+// bf16 in 829 us (5.1 TB/s).  Read a second time instead: 1280 us with four times as many rows on the
 // way as the last-level cache holds, 950 us with as many as it does hold.
 template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillArgs a) {
   constexpr int N = Elem<DT>::N;
@@ -649,10 +650,10 @@ template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) 
 // The gradient from the pair (m, log S) that the loss left, in two launches: all elements as if the
 // teacher named none of them, a vector a thread in memory order, then a workgroup a row for those
 // that it does name (and for rows where it names none at all, whose gradient is 0).
-template <int DT> __global__ __launch_bounds__(256) void distill_stream(DistillArgs a, int spans) {
+template <int DT> __global__ __launch_bounds__(256) void distill_stream(DistillArgs a, int spans, int64_t row0) {
   constexpr int N = Elem<DT>::N;
   typedef typename Elem<DT>::T T;
-  const int64_t row = blockIdx.x / spans;
+  const int64_t row = row0 + blockIdx.x / spans;
   const int at = (static_cast<int>(blockIdx.x % spans) * 256 + static_cast<int>(threadIdx.x)) * N, n = a.in.vocab - at;
   if (n <= 0) return;
   const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride + at;
@@ -780,12 +781,21 @@ template <class F> hipError_t by_items(int items, F&& f) {
   }
 }
 unsigned grid_of(int64_t n) { return static_cast<unsigned>(n); }
+// `spans` workgroups for each row, in launches of as many rows as one can have.
+template <class F> hipError_t by_row_runs(int64_t rows, int spans, F&& f) {
+  const int64_t run = kLaunchBlocks / spans;
+  for (int64_t row0 = 0; row0 < rows; row0 += run) {
+    f(row0, grid_of((rows - row0 < run ? rows - row0 : run) * spans));
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
 
 template <int DT> hipError_t launch_gradient_alone(const DistillArgs& a, hipStream_t stream) {
   constexpr int span = 256 * Elem<DT>::N;
   const int spans = (a.in.vocab + span - 1) / span;
-  distill_stream<DT><<<grid_of(a.in.rows * spans), 256, 0, stream>>>(a, spans);
-  if (hipError_t e = hipGetLastError()) return e;
+  const hipError_t e = by_row_runs(a.in.rows, spans, [&](int64_t row0, unsigned grid) { distill_stream<DT><<<grid, 256, 0, stream>>>(a, spans, row0); });
+  if (e != hipSuccess) return e;
   if (a.k <= 64) distill_named<DT, 64><<<grid_of(a.in.rows), 64, Teacher::bytes(a.k, 64), stream>>>(a);
   else distill_named<DT, 256><<<grid_of(a.in.rows), 256, Teacher::bytes(a.k, 256), stream>>>(a);
   return hipGetLastError();
@@ -824,9 +834,10 @@ hipError_t launch_score_grad(const ScoreGradArgs& a, hipStream_t stream) {
   return by_type(a.in.dtype, [&](auto dt) {
     constexpr int span = 256 * Elem<dt.value>::N;
     const int spans = (a.in.vocab + span - 1) / span;
-    if (a.grad_entropy) score_grad_rows<dt.value, true><<<grid_of(a.in.rows * spans), 256, 0, stream>>>(a, spans);
-    else score_grad_rows<dt.value, false><<<grid_of(a.in.rows * spans), 256, 0, stream>>>(a, spans);
-    return hipGetLastError();
+    return by_row_runs(a.in.rows, spans, [&](int64_t row0, unsigned grid) {
+      if (a.grad_entropy) score_grad_rows<dt.value, true><<<grid, 256, 0, stream>>>(a, spans, row0);
+      else score_grad_rows<dt.value, false><<<grid, 256, 0, stream>>>(a, spans, row0);
+    });
   });
 }
 

@@ -237,15 +237,22 @@ void check_sequences(int64_t batch, int64_t time, int64_t width) {
   if (batch < 0 || batch > (int64_t{1} << 22)) throw Error("batch: " + std::to_string(batch) + " is out of range (0 to 2^22)");
   if (time < 0 || time > (int64_t{1} << 31)) throw Error("time: " + std::to_string(time) + " is out of range (0 to 2^31)");
   if (width < 1 || width > (int64_t{1} << 24)) throw Error("width: " + std::to_string(width) + " is out of range (1 to 2^24)");
-  if (batch * width > (int64_t{1} << 34)) throw Error("batch, width: " + std::to_string(batch) + " sequences of " + std::to_string(width) + " channels are out of range (2^34 together)");
+  if (batch * width > (int64_t{1} << 33)) throw Error("batch, width: " + std::to_string(batch) + " sequences of " + std::to_string(width) + " channels are out of range (2^33 together)");
 }
 
 int units(const HipDevice& d) { return std::max(d.profile().compute_units, 1); }
 
+// A launch's threads are counted in 32 bits.
+void check_threads(int64_t blocks, int threads, const char* what) {
+  if (blocks > ((int64_t{1} << 32) - 1) / threads) throw Error(std::string(what) + ": out of range together, a launch cannot count the threads");
+}
+
 RowSplit split_of(const HipDevice& d, int64_t rows, int64_t vocab, const eh_array& logits, bool top) {
   if (!is_float(logits.dtype)) throw Error("logits: has to be f32, bf16 or f16");
   if (rows == 0) return {64, 0, 1, static_cast<int>(vocab)};
-  return split_rows(rows, static_cast<int>(vocab), static_cast<int>(logits.dtype), top, units(d));
+  const RowSplit s = split_rows(rows, static_cast<int>(vocab), static_cast<int>(logits.dtype), top, units(d));
+  check_threads(rows * s.segs, s.threads, "rows, vocab");
+  return s;
 }
 
 void check_top(const eh_token_logprobs_args* a) {
@@ -270,6 +277,11 @@ Sequences sequences(Arrays& arrays, const char* name, const eh_array& a, int64_t
   s.batch = a.stride[0];
   s.step = a.stride[1];
   return s;
+}
+
+void check_plan(const ScanArgs& s) {
+  const ScanPlan p = plan_scan(s);
+  if (p.waves) check_threads(s.batch * p.tiles * p.pieces, 64 * p.waves, "batch, time, width");
 }
 
 #define REQUIRE(cond, msg) \
@@ -299,6 +311,7 @@ int eh_token_logprobs(eh_device* dev, const eh_token_logprobs_args* args, int sy
     Current current(d);
     Arrays arrays(d);
     ScoreArgs s{};
+    s.split = split_of(*d, a.rows, a.vocab, a.logits, a.top > 0);
     s.in = logit_rows(arrays, a.logits, a.rows, a.vocab, check_scale(a.scale, "scale"));
     s.targets = arrays.ids("targets", a.targets, a.rows, 1);
     if (a.targets.stride[0] != 1 && a.rows > 1) bad("targets", "has to be contiguous");
@@ -311,7 +324,6 @@ int eh_token_logprobs(eh_device* dev, const eh_token_logprobs_args* args, int sy
       s.top_logp = arrays.small<float>("top_logp", a.top_logp, a.rows, a.top, EH_F32, true, true);
       s.top_ids = arrays.small<int>("top_ids", a.top_ids, a.rows, a.top, EH_I32, true, true);
     }
-    s.split = split_of(*d, a.rows, a.vocab, a.logits, a.top > 0);
     Workspace ws(d, arrays, a.workspace, split_workspace(s.split, a.rows, s.top));
     s.workspace = ws.at();
     arrays.settle();
@@ -364,6 +376,7 @@ static void distill(eh_device* dev, const eh_distill_loss_args& a, bool backward
   Current current(d);
   Arrays arrays(d);
   DistillArgs s{};
+  s.split = split_of(*d, a.rows, a.vocab, a.logits, false);
   s.temperature = check_scale(a.temperature, "temperature");
   s.in = logit_rows(arrays, a.logits, a.rows, a.vocab, 1.f / s.temperature);
   s.teacher = arrays.floats("teacher", a.teacher, a.rows, 1, a.k, -1, false);
@@ -379,8 +392,8 @@ static void distill(eh_device* dev, const eh_distill_loss_args& a, bool backward
     s.grad = arrays.floats("grad", a.grad, a.rows, 1, a.vocab, a.logits.dtype, true);
     s.grad_stride = a.grad.stride[0];
   }
-  s.split = split_of(*d, a.rows, a.vocab, a.logits, false);
   s.held = hold_rows(a.rows, s.in.vocab, s.in.dtype, units(*d));
+  if (s.grad) check_threads(a.rows, backward ? 256 : s.held.threads, "rows, vocab");
   const eh_array none{};
   Workspace ws(d, arrays, backward ? none : a.workspace, backward ? 0 : split_workspace(s.split, a.rows, 0));
   s.workspace = ws.at();
@@ -451,6 +464,7 @@ int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync) {
     s.state = arrays.small<const float>("state", a.state, a.batch, a.width, EH_F32, false, false);
     s.final_state = arrays.small<float>("final_state", a.final_state, a.batch, a.width, EH_F32, false, true);
     s.lengths = arrays.small<const int>("lengths", a.lengths, a.batch, 1, EH_I32, false, false);
+    check_plan(s);
     Workspace ws(d, arrays, a.workspace, scan_workspace(s));
     s.workspace = ws.at();
     arrays.settle();
@@ -479,6 +493,7 @@ int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* ar
     s.grad_final = arrays.small<const float>("grad_final", a.grad_final, a.batch, a.width, EH_F32, false, false);
     s.final_state = arrays.small<float>("grad_state", a.grad_state, a.batch, a.width, EH_F32, false, true);
     s.lengths = arrays.small<const int>("lengths", a.lengths, a.batch, 1, EH_I32, false, false);
+    check_plan(s);
     Workspace ws(d, arrays, a.workspace, scan_workspace(s));
     s.workspace = ws.at();
     arrays.settle();

@@ -41,6 +41,8 @@ struct RowSplit {
   int segs;
   int seg;
 };
+// A launch's threads are counted in 32 bits: most workgroups of 256 in one.
+constexpr int64_t kLaunchBlocks = (int64_t{1} << 24) - 1;
 RowSplit split_rows(int64_t rows, int vocab, int dtype, bool top, int compute_units);
 // What a segment leaves for the join (its best keys, 8 bytes each, follow).
 struct RowPartial {

@@ -215,6 +215,7 @@ static void scores(eh_device* d, eh_device* other) {
   bad([](auto& a) { a.vocab = 0; }, "vocab");
   bad([](auto& a) { a.vocab = int64_t{1} << 31; }, "vocab");
   bad([](auto& a) { a.rows = 1 << 24, a.vocab = 1 << 30; }, "out of range together");
+  bad([](auto& a) { a.rows = 1 << 23, a.vocab = 1 << 17; }, "out of range together");
   bad([](auto& a) { a.top = -1; }, "top");
   bad([](auto& a) { a.top = 33; }, "top");
   bad([](auto& a) { a.vocab = 3; }, "top");
@@ -353,7 +354,7 @@ static void recurrences(eh_device* d) {
   bad([](auto& a) { a.time = -1; }, EH_ERR_INVALID, "time");
   bad([](auto& a) { a.width = 0; }, EH_ERR_INVALID, "width");
   bad([](auto& a) { a.batch = 1 << 22, a.width = 1 << 24; }, EH_ERR_INVALID, "batch, width");
-  bad([](auto& a) { a.batch = 1 << 22, a.width = 4096, a.time = int64_t{1} << 31; }, EH_ERR_INVALID, "out of range together");
+  bad([](auto& a) { a.batch = 1 << 22, a.width = 2048, a.time = int64_t{1} << 31; }, EH_ERR_INVALID, "out of range together");
   bad([](auto& a) { a.x.dtype = EH_F32; }, EH_ERR_INVALID, "other arrays' type");
   bad([](auto& a) { a.out = a.x; }, EH_ERR_INVALID, "overlap");
   bad([](auto& a) { a.out.stride[1] = 9; }, EH_ERR_INVALID, "rows overlap");

@@ -654,6 +654,33 @@ def test_rows_far_apart_in_a_large_array(dev, ops, dtype):
     close(host(out), h, tol + oracle.rounding(dtype, h), "h")
 
 
+def test_gradients_of_more_vectors_than_a_launch_has_threads(dev, ops):
+    """2^32 vectors and more of one gradient (69 GB, of a row that all share): every row has the same."""
+    n, v = 262150, 131072
+    row = rows_of(1, v, "bf16", 4)
+    z, out = row.expand(n, v), torch.empty(n, v, device="cuda", dtype=torch.bfloat16)
+    t = torch.full((1,), 77, device="cuda")
+    score = ops.Logprobs(*(torch.empty(1, device="cuda") for _ in range(2)), torch.empty(1, 2, device="cuda"), None, None)
+    ops.token_logprobs(dev, row, t, out=score)
+    e = torch.full((n,), 0.5, device="cuda")
+    one = torch.empty(1, v, device="cuda", dtype=torch.bfloat16)
+
+    def same(want):
+        assert not bool(torch.isnan(want).any())
+        for lo in range(0, n, 8192):
+            assert bool((out[lo:lo + 8192] == want).all()), lo
+        out.fill_(float("nan"))
+    ops.token_logprobs_backward(dev, row, t, score.norm, score.entropy, e[:1], e[:1], out=one)
+    ops.token_logprobs_backward(dev, z, t.expand(n).contiguous(), score.norm.expand(n, 2).contiguous(), score.entropy.expand(n).contiguous(), e, e, out=out)
+    same(one)
+    u, ids = torch.zeros(1, 2, device="cuda"), torch.tensor([[5, v - 1]], device="cuda")
+    loss = ops.Distilled(torch.empty(1, device="cuda"), torch.empty(1, 2, device="cuda"), None)
+    ops.distill_loss(dev, row, u, ids, out=loss)
+    ops.distill_loss_backward(dev, row, u, ids, loss.norm, out=one)
+    ops.distill_loss_backward(dev, z, u.expand(n, 2), ids.expand(n, 2), loss.norm.expand(n, 2).contiguous(), out=out)
+    same(one)
+
+
 REFUSED = [
     ("overlap", lambda o, d, z, t, e: o.token_logprobs_backward(d, z, t, e(4, 2), out=z)),
     ("overlap", lambda o, d, z, t, e: o.gated_scan(d, z[None], z[None], out=z[None])),
