@@ -41,6 +41,16 @@ __device__ inline unsigned int word_of(float x) {
   return b == kEmpty ? 0x7fc00000u : b;
 }
 
+// A word of the board once it is there.  That every wait ends follows from the order of the tickets; one that
+// has lasted for seconds all the same (two calls in one workspace at once, say) ends with the
+// empty word, which is NaN.
+template <class Word> __device__ inline Word wait_for(const Word* p) {
+  Word w;
+  for (int i = 0; (w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == static_cast<Word>(~0ull) && i < 1 << 22; ++i)
+    __builtin_amdgcn_s_sleep(1);
+  return w;
+}
+
 // A row of at least a vector is read by the vector that ends with it, which `down` channels are moved out of: by
 // whole words, then by half a one.  32 bits at a time, since a 64-bit shift whose amount is in the last
 // register that a kernel has was seen to take v0's value for it now and then (the gradient of 13 x 1999 x 717
@@ -285,9 +295,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     if (p == 0 && mine && behind < last && member < P - 1)
       __hip_atomic_store(words, static_cast<unsigned long long>(word_of(ma)) << 32 | word_of(mb), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (mine && p < member) {
-      unsigned long long w;
-      while ((w = __hip_atomic_load(words - static_cast<int64_t>(member - p) * CW, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == ~0ull)
-        __builtin_amdgcn_s_sleep(1);
+      const unsigned long long w = wait_for(words - static_cast<int64_t>(member - p) * CW);
       others[0][p][c] = __uint_as_float(static_cast<unsigned int>(w >> 32));
       others[1][p][c] = __uint_as_float(static_cast<unsigned int>(w));
     }
@@ -297,10 +305,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     if (behind < P) {
       h = start ? start[b * a.width + tile + c] : 0.f;
     } else {
-      unsigned int w;
-      while ((w = __hip_atomic_load(board.states + (group - 1) * CW + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == kEmpty)
-        __builtin_amdgcn_s_sleep(1);
-      h = __uint_as_float(w);
+      h = __uint_as_float(wait_for(board.states + (group - 1) * CW + c));
     }
     before[c] = h;
   }

@@ -306,8 +306,8 @@ typedef struct eh_token_logprobs_args {
 int eh_token_logprobs(eh_device* dev, const eh_token_logprobs_args* args, int sync);
 /* Bytes of device memory that the call needs besides its arrays: 0 where a row is a workgroup's
  * work, partial sums where few long rows are split.  Without a `workspace` array the call takes them
- * from the device's pool; under stream capture it must be given, and graphs whose replays may
- * overlap need one each. */
+ * from the device's pool; under stream capture it must be given.  One call at a time works in a
+ * workspace: graphs whose replays may overlap need one each (results of such calls are undefined). */
 int eh_token_logprobs_workspace(eh_device* dev, const eh_token_logprobs_args* args, size_t* bytes);
 
 /* The gradient with respect to the logits of sum_r (grad_logp_r logp_r + grad_entropy_r entropy_r):
