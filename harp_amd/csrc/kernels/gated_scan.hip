@@ -232,6 +232,14 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     load_steps<DT, FAR>({a.gate, b, k * RUN, tile}, row, rows - 1, cb, nc, a.width, vg);
     load_steps<DT, FAR>({BACK ? a.out : a.x, b, k * RUN, tile}, row, rows - 1, cb, nc, a.width, vx);
   }
+  // the backward pass: h of the step before each, the rows from the piece before's last on; the first step of all has
+  // the state.  Loaded with the rest where a workgroup has the registers, with half of them once the gates are through.
+  u32x4 vh[BACK ? kSteps : 1];
+  auto load_states = [&] {
+    const int first = k > 0 ? 1 : 0;
+    if (n > 0 && nc > 0) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, a.width, vh);
+  };
+  if constexpr (BACK && EU == 2) load_states();
   float A[N], B[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) A[j] = 1.f, B[j] = 0.f;
@@ -344,10 +352,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     }
   } else {
     const PieceRows<DT, FAR> dg(a.grad_gate, b, k * RUN, tile), dx(a.grad_x, b, k * RUN, tile);
-    u32x4 vh[kSteps];
-    // h of the step before each: the rows from the piece before's last on; the first step of all has the state
-    const int first = k > 0 ? 1 : 0;
-    if (n > 0) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, a.width, vh);
+    if constexpr (EU != 2) load_states();
 #pragma unroll
     for (int i = kSteps - 1; i >= 0; --i) {
       if (row + i >= rows) continue;                                       // h stays what came from behind
@@ -510,6 +515,9 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
     if (p.far) return go(std::integral_constant<int, 8>{}, std::true_type{}, two);
     if (p.waves == 1) return go(std::integral_constant<int, 1>{}, std::false_type{}, two);
     if (p.waves == 4) return go(std::integral_constant<int, 4>{}, std::false_type{}, two);
+    if constexpr (BACK && dt.value != kF32) {
+      if (p.wide) return go(std::integral_constant<int, 8>{}, std::false_type{}, two);
+    }
     return go(std::integral_constant<int, 8>{}, std::false_type{}, std::integral_constant<int, 4>{});
   });
 }

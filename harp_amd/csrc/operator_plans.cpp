@@ -63,6 +63,10 @@ static bool on_lines(const Sequences& s, const ScanArgs& a) {
 
 // Sequences of a few steps by a thread each, where that fills the device (1024 x 9 x 2048 bf16 20 us against 69
 // with a piece's 64 steps for each, 64 x 16 x 2048 8 us against 8.5, from 32 steps on no difference).
+// Wide: one workgroup on a compute unit instead of two, us a gradient with and without, by workgroups of a compute unit:
+//   one    4 x 1999 x 717 f16 19.3 : 20.5       two   4 x 4096 x 1024 bf16 38 : 34, 32 x 512 x 704 f16 27 : 21
+//   eight  8 x 4096 x 2048 bf16 136 : 145       more  64 x 4096 x 1024 bf16 496 : 537, 52 x 2048 x 717 f16 210 : 222
+// (in f32, which needs fewer registers, 161 : 156 and 497 : 502)
 ScanPlan plan_scan(const ScanArgs& a) {
   ScanPlan p{};
   int64_t step = 0;
@@ -80,6 +84,8 @@ ScanPlan plan_scan(const ScanArgs& a) {
   for (const Sequences* s : {&a.gate, &a.x, &a.out, &a.grad_gate, &a.grad_x})
     if (s->p) lines = lines && on_lines(*s, a);
   p.classes = lines ? 1 : 8;
+  const int64_t blocks = a.batch * p.tiles * p.pieces;
+  p.wide = blocks <= a.compute_units || blocks >= 8 * static_cast<int64_t>(a.compute_units);
   return p;
 }
 

@@ -421,10 +421,11 @@ int eh_distill_loss_backward(eh_device* dev, const eh_distill_loss_args* args, i
   });
 }
 
-static ScanArgs scan_sizes(int64_t batch, int64_t time, int64_t width, int64_t log_gate, const eh_array& gate) {
+static ScanArgs scan_sizes(const HipDevice& d, int64_t batch, int64_t time, int64_t width, int64_t log_gate, const eh_array& gate) {
   check_sequences(batch, time, width);
   if (!is_float(gate.dtype)) throw Error("gate: has to be f32, bf16 or f16");
   ScanArgs s{};
+  s.compute_units = units(d);
   s.batch = batch, s.time = time, s.width = static_cast<int>(width);
   s.dtype = static_cast<int>(gate.dtype);
   s.log_gate = log_gate != 0;
@@ -437,14 +438,14 @@ static ScanArgs scan_sizes(int64_t batch, int64_t time, int64_t width, int64_t l
 int eh_gated_scan_workspace(eh_device* dev, const eh_gated_scan_args* args, size_t* bytes) {
   REQUIRE(dev && args && bytes, "device, args or bytes is NULL");
   return guard([&] {
-    *bytes = scan_workspace(scan_sizes(args->batch, args->time, args->width, args->log_gate, args->gate));
+    *bytes = scan_workspace(scan_sizes(dev->dev, args->batch, args->time, args->width, args->log_gate, args->gate));
   });
 }
 
 int eh_gated_scan_backward_workspace(eh_device* dev, const eh_gated_scan_backward_args* args, size_t* bytes) {
   REQUIRE(dev && args && bytes, "device, args or bytes is NULL");
   return guard([&] {
-    *bytes = scan_workspace(scan_sizes(args->batch, args->time, args->width, args->log_gate, args->gate));
+    *bytes = scan_workspace(scan_sizes(dev->dev, args->batch, args->time, args->width, args->log_gate, args->gate));
   });
 }
 
@@ -453,7 +454,7 @@ int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync) {
   return guard([&] {
     const eh_gated_scan_args& a = *args;
     HipDevice* d = &dev->dev;
-    ScanArgs s = scan_sizes(a.batch, a.time, a.width, a.log_gate, a.gate);
+    ScanArgs s = scan_sizes(*d, a.batch, a.time, a.width, a.log_gate, a.gate);
     auto lk = d->stream_lock();
     Current current(d);
     Arrays arrays(d);
@@ -479,7 +480,7 @@ int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* ar
   return guard([&] {
     const eh_gated_scan_backward_args& a = *args;
     HipDevice* d = &dev->dev;
-    ScanArgs s = scan_sizes(a.batch, a.time, a.width, a.log_gate, a.gate);
+    ScanArgs s = scan_sizes(*d, a.batch, a.time, a.width, a.log_gate, a.gate);
     auto lk = d->stream_lock();
     Current current(d);
     Arrays arrays(d);

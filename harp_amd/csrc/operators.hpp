@@ -123,6 +123,7 @@ struct ScanArgs {
   float* final_state;          // [batch][width] or null; gradients: the gradient of `state`
   const float* grad_final;     // gradients only, or null
   const int* lengths;          // [batch] or null
+  int compute_units;
   void* workspace;
 };
 // A workgroup of `waves` waves has kScanLanes vectors of channels and a piece of waves * 64 steps.
@@ -135,6 +136,7 @@ struct ScanPlan {
   int64_t pieces, tiles;             // of a sequence, of a row
   int64_t per_group, groups;         // pieces whose maps are composed from one state
   int classes;                       // of columns, see the kernel
+  bool wide;                         // gradients in 16 bits: all of a thread's loads at once, in twice the registers
 };
 ScanPlan plan_scan(const ScanArgs& a);
 constexpr size_t kTicketBytes = 256;

@@ -396,6 +396,8 @@ def test_scan_layouts(dev, ops, layout, dtype):
 def test_scan_last_channels(dev, ops, dtype, log_gate):
     """Rows that end inside a vector, in many workgroups at once: with every count of channels in the last one."""
     check_scan(dev, ops, 6, 1030, 717, dtype, log_gate, lengths=[1030, 1, 513, 1029, 700, 1030])
+    check_scan(dev, ops, 16, 600, 717, dtype, log_gate)       # (more workgroups than the device runs one a compute unit)
+    check_scan(dev, ops, 5, 1100, 1408, dtype, log_gate)
     for width in (65, 74, 83, 92, 102, 111):
         check_scan(dev, ops, 3, 530, width, dtype, log_gate)
 
