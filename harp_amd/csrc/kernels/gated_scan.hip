@@ -173,9 +173,12 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 // pieces, so all are taken.
 //
 // With eight classes, by the workgroup's number, neighbouring columns are read and written behind one
-// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes 38 us
-// instead of 44 (64 x 512 x 1000 f32 84 instead of 104).  Where they do start there, one class is better
-// (8 x 4096 x 2048 bf16 87 us instead of 91 to 102).
+// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes 31 us
+// instead of 36 (its gradient 50 instead of 60, 64 x 512 x 1000 f32 85 instead of 106).  Where they do start
+// there, one class is better (8 x 4096 x 2048 bf16 88 us instead of 92, the gradient 136 instead of 146).
+//
+// Bound by memory: 8 x 4096 x 2048 bf16 at 4.6 TB/s forward and 4.9 backward, 1 x 131072 x 512 f32 at 5.4.  Smaller
+// pieces read the same at more waits and shares of the board, two vectors a lane do not fit the registers.
 // a wave has 64 steps, which the plan's choice of waves goes by, and a workgroup a thread per channel
 static_assert(64 / kLanes * kSteps == 64 && kLanes * 8 <= 64);
 template <int DT, int W, bool BACK, bool LOG, bool FAR, int EU>
