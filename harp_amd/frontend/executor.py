@@ -134,6 +134,8 @@ def _run_operators(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
         for n in nodes:
             if key(n) not in values and n not in todo:
                 if n.is_external() and n.view == View.contiguous(n.shape()):
+                    if id(n) not in buffers:
+                        raise ExecutionError(f"MissingInput: {n.name or hex(id(n))}, read by an operator")
                     values[key(n)] = n
                 else:
                     todo.append(n)

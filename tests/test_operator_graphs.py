@@ -213,6 +213,13 @@ def test_refused_shapes_and_types(fe, bad):
         bad(fe, z, t, tensor(fe, np.zeros((2, 3, 4), np.float32)))
 
 
+def test_an_input_without_a_buffer(fe):
+    from harp_amd.frontend.executor import ExecutionError, execute_graph
+    logp, _ = fe.nn.token_logprobs(fe.Tensor.input([2, 3], fe.F32), fe.Tensor.input([2], fe.DType("i64")))
+    with pytest.raises(ExecutionError, match="MissingInput"):
+        execute_graph([logp.graph], {})
+
+
 def test_programs_and_backends_without_operators(fe):
     from harp_amd.frontend.lowerer import LoweringError, lower_graph
     s = tensor(fe, np.ones((1, 2, 3), np.float32))
