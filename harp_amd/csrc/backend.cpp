@@ -22,8 +22,9 @@ namespace eh {
 namespace {
 
 void check(hipError_t e, const char* what) {
-  if (e != hipSuccess)
-    throw Error(std::string(what) + ": " + hipGetErrorString(e) + " (hip error " + std::to_string(static_cast<int>(e)) + ")");
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();             // reported here, and not a second time by the thread's next caller of HIP
+  throw Error(std::string(what) + ": " + hipGetErrorString(e) + " (hip error " + std::to_string(static_cast<int>(e)) + ")");
 }
 
 uint64_t fnv1a(const std::string& s, uint64_t h) {
@@ -402,6 +403,7 @@ HipKernel::HipKernel(HipDevice* dev, const Binary& bin, const std::string& entry
   hipError_t e = hipModuleGetFunction(&fn_, module_, entry.c_str());
   if (e != hipSuccess) {
     (void)hipModuleUnload(module_);
+    (void)hipGetLastError();
     module_ = nullptr;
     throw Error("entry point '" + entry + "' not found in the code object: " + hipGetErrorString(e));
   }

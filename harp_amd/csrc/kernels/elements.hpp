@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <tuple>
 
 #include "../operators.hpp"
 
@@ -144,6 +145,22 @@ __device__ inline float wave_max(float x) {
   x = fmaxf(x, dpp<kBcast15, 0xa>(x, x));
   x = fmaxf(x, dpp<kBcast31, 0xc>(x, x));
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+
+// Queues a kernel and returns what the launch itself returns: the thread's last error may be an earlier call's, of
+// anybody's.  An error that is returned here is not left there.
+template <class... P, class... A>
+hipError_t queue(void (*kernel)(P...), unsigned grid, int threads, size_t lds, hipStream_t stream, const A&... args) {
+  static_assert(sizeof...(P) == sizeof...(A));
+  std::tuple<P...> values(static_cast<P>(args)...);
+  const hipError_t e = std::apply(
+      [&](auto&... v) {
+        void* list[] = {static_cast<void*>(&v)...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(static_cast<unsigned>(threads)), list, lds, stream);
+      },
+      values);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
 }
 
 // The same over a workgroup of THREADS; `lds` holds a value per wave and is free again afterwards.

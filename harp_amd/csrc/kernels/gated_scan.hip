@@ -486,11 +486,10 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
   if (p.waves == 0) {
     return by_type(a.dtype, [&](auto dt) {
       const int vectors = (a.width + Elem<dt.value>::N - 1) / Elem<dt.value>::N;
-      const dim3 grid(static_cast<unsigned>((a.batch * vectors + 255) / 256));
+      const unsigned grid = static_cast<unsigned>((a.batch * vectors + 255) / 256);
       auto go = [&](auto steps) {
-        if (a.log_gate) scan_short<dt.value, steps.value, BACK, true><<<grid, 256, 0, stream>>>(a, vectors);
-        else scan_short<dt.value, steps.value, BACK, false><<<grid, 256, 0, stream>>>(a, vectors);
-        return hipGetLastError();
+        return a.log_gate ? queue(scan_short<dt.value, steps.value, BACK, true>, grid, 256, 0, stream, a, vectors)
+                          : queue(scan_short<dt.value, steps.value, BACK, false>, grid, 256, 0, stream, a, vectors);
       };
       if (a.time <= 1) return go(std::integral_constant<int, 1>{});
       return go(std::integral_constant<int, kSteps>{});
@@ -503,16 +502,14 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
     board.maps = reinterpret_cast<unsigned long long*>(board.tickets + kTicketBytes / 4);
     board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.pieces * p.channels);
     const size_t blocks = (words + 1023) / 1024;
-    clear_board<<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), 256, 0, stream>>>(board.tickets, words);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = queue(clear_board, static_cast<unsigned>(blocks < 1024 ? blocks : 1024), 256, 0, stream, board.tickets, words)) return e;
   }
-  const dim3 grid(static_cast<unsigned>(a.batch * p.tiles * p.pieces));
+  const unsigned grid = static_cast<unsigned>(a.batch * p.tiles * p.pieces);
   return by_type(a.dtype, [&](auto dt) {
     auto go = [&](auto waves, auto is_far, auto eu) {
       const int pieces = static_cast<int>(p.pieces), tiles = static_cast<int>(p.tiles);
-      if (a.log_gate) scan_pieces<dt.value, waves.value, BACK, true, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, p.classes, board);
-      else scan_pieces<dt.value, waves.value, BACK, false, is_far.value, eu.value><<<grid, 64 * waves.value, 0, stream>>>(a, pieces, tiles, p.classes, board);
-      return hipGetLastError();
+      return a.log_gate ? queue(scan_pieces<dt.value, waves.value, BACK, true, is_far.value, eu.value>, grid, 64 * waves.value, 0, stream, a, pieces, tiles, p.classes, board)
+                        : queue(scan_pieces<dt.value, waves.value, BACK, false, is_far.value, eu.value>, grid, 64 * waves.value, 0, stream, a, pieces, tiles, p.classes, board);
     };
     const std::integral_constant<int, 2> two;
     if (p.far) return go(std::integral_constant<int, 8>{}, std::true_type{}, two);

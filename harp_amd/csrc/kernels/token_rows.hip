@@ -785,8 +785,7 @@ unsigned grid_of(int64_t n) { return static_cast<unsigned>(n); }
 template <class F> hipError_t by_row_runs(int64_t rows, int spans, F&& f) {
   const int64_t run = kLaunchBlocks / spans;
   for (int64_t row0 = 0; row0 < rows; row0 += run) {
-    f(row0, grid_of((rows - row0 < run ? rows - row0 : run) * spans));
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = f(row0, grid_of((rows - row0 < run ? rows - row0 : run) * spans))) return e;
   }
   return hipSuccess;
 }
@@ -794,11 +793,10 @@ template <class F> hipError_t by_row_runs(int64_t rows, int spans, F&& f) {
 template <int DT> hipError_t launch_gradient_alone(const DistillArgs& a, hipStream_t stream) {
   constexpr int span = 256 * Elem<DT>::N;
   const int spans = (a.in.vocab + span - 1) / span;
-  const hipError_t e = by_row_runs(a.in.rows, spans, [&](int64_t row0, unsigned grid) { distill_stream<DT><<<grid, 256, 0, stream>>>(a, spans, row0); });
+  const hipError_t e = by_row_runs(a.in.rows, spans, [&](int64_t row0, unsigned grid) { return queue(distill_stream<DT>, grid, 256, 0, stream, a, spans, row0); });
   if (e != hipSuccess) return e;
-  if (a.k <= 64) distill_named<DT, 64><<<grid_of(a.in.rows), 64, Teacher::bytes(a.k, 64), stream>>>(a);
-  else distill_named<DT, 256><<<grid_of(a.in.rows), 256, Teacher::bytes(a.k, 256), stream>>>(a);
-  return hipGetLastError();
+  if (a.k <= 64) return queue(distill_named<DT, 64>, grid_of(a.in.rows), 64, Teacher::bytes(a.k, 64), stream, a);
+  return queue(distill_named<DT, 256>, grid_of(a.in.rows), 256, Teacher::bytes(a.k, 256), stream, a);
 }
 
 }  // namespace
@@ -810,17 +808,15 @@ hipError_t launch_score(const ScoreArgs& a, hipStream_t stream) {
         if (a.split.held) {
           return by_items(a.split.held, [&](auto items) {
             if constexpr (held_form(threads.value, items.value))
-              score_held<dt.value, threads.value, items.value, ent.value><<<grid_of(a.in.rows), threads.value, 0, stream>>>(a);
-            return hipGetLastError();
+              return queue(score_held<dt.value, threads.value, items.value, ent.value>, grid_of(a.in.rows), threads.value, 0, stream, a);
+            else return hipErrorInvalidValue;
           });
         }
       }
-      score_rows<dt.value, threads.value, ent.value, top.value><<<grid_of(a.in.rows * a.split.segs), threads.value, 0, stream>>>(a);
-      return hipGetLastError();
+      return queue(score_rows<dt.value, threads.value, ent.value, top.value>, grid_of(a.in.rows * a.split.segs), threads.value, 0, stream, a);
     });
     if (e != hipSuccess || a.split.segs == 1) return e;
-    score_join<256, ent.value, top.value><<<grid_of(a.in.rows), 256, 0, stream>>>(a);
-    return hipGetLastError();
+    return queue(score_join<256, ent.value, top.value>, grid_of(a.in.rows), 256, 0, stream, a);
   };
   return by_type(a.in.dtype, [&](auto dt) {
     const std::true_type yes;
@@ -835,8 +831,8 @@ hipError_t launch_score_grad(const ScoreGradArgs& a, hipStream_t stream) {
     constexpr int span = 256 * Elem<dt.value>::N;
     const int spans = (a.in.vocab + span - 1) / span;
     return by_row_runs(a.in.rows, spans, [&](int64_t row0, unsigned grid) {
-      if (a.grad_entropy) score_grad_rows<dt.value, true><<<grid, 256, 0, stream>>>(a, spans, row0);
-      else score_grad_rows<dt.value, false><<<grid, 256, 0, stream>>>(a, spans, row0);
+      if (a.grad_entropy) return queue(score_grad_rows<dt.value, true>, grid, 256, 0, stream, a, spans, row0);
+      return queue(score_grad_rows<dt.value, false>, grid, 256, 0, stream, a, spans, row0);
     });
   });
 }
@@ -850,20 +846,16 @@ hipError_t launch_distill(const DistillArgs& a, hipStream_t stream) {
     constexpr int DT = dt.value;
     const unsigned rows = grid_of(a.in.rows);
     if (a.split.segs > 1) {
-      distill_parts<DT, 512><<<grid_of(a.in.rows * a.split.segs), 512, 0, stream>>>(a);
-      if (hipError_t e = hipGetLastError()) return e;
-      distill_join<DT, 256><<<rows, 256, Teacher::bytes(a.k, 256), stream>>>(a);
-      hipError_t e = hipGetLastError();
+      if (hipError_t e = queue(distill_parts<DT, 512>, grid_of(a.in.rows * a.split.segs), 512, 0, stream, a)) return e;
+      const hipError_t e = queue(distill_join<DT, 256>, rows, 256, Teacher::bytes(a.k, 256), stream, a);
       return e != hipSuccess || !a.grad ? e : launch_gradient_alone<DT>(a, stream);
     }
     if (!a.grad)
       return by_threads(a.split.threads, [&](auto threads) {
-        distill_rows<DT, threads.value, false><<<rows, threads.value, Teacher::bytes(a.k, threads.value), stream>>>(a);
-        return hipGetLastError();
+        return queue(distill_rows<DT, threads.value, false>, rows, threads.value, Teacher::bytes(a.k, threads.value), stream, a);
       });
     auto held = [&](auto threads, auto nv) {
-      distill_held<DT, threads.value, nv.value><<<rows, threads.value, Teacher::bytes(a.k, threads.value), stream>>>(a);
-      return hipGetLastError();
+      return queue(distill_held<DT, threads.value, nv.value>, rows, threads.value, Teacher::bytes(a.k, threads.value), stream, a);
     };
     const std::integral_constant<int, 4> four;
     const std::integral_constant<int, 16> sixteen;
@@ -879,8 +871,7 @@ hipError_t launch_distill(const DistillArgs& a, hipStream_t stream) {
       if (a.held.threads == 512) return held(std::integral_constant<int, 512>{}, sixteen);
       return held(t1024, sixteen);
     }
-    distill_rows<DT, 1024, true><<<rows, 1024, Teacher::bytes(a.k, 1024), stream>>>(a);
-    return hipGetLastError();
+    return queue(distill_rows<DT, 1024, true>, rows, 1024, Teacher::bytes(a.k, 1024), stream, a);
   });
 }
 

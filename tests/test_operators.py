@@ -656,6 +656,19 @@ def test_rows_far_apart_in_a_large_array(dev, ops, dtype):
     close(host(out), h, tol + oracle.rounding(dtype, h), "h")
 
 
+def test_an_earlier_calls_error_is_reported_once(dev, ops):
+    """A refused call of HIP leaves its error with the thread: neither an operator nor another library takes it for its own."""
+    from harp_amd import backend as hb
+    from harp_amd import frontend as fe
+    a = fe.Tensor.input([256])
+    blob = hb.HipKernel(dev, fe.lower_graph([(a * a).graph])[0]).get_binary()
+    z, t = rows_of(4, 30, "f32", 0), on_gpu(np.array([1, 2, 3, 4]))
+    for after in (lambda: check_score(dev, ops, z, t), lambda: torch.ones(3, device="cuda").sum().item()):
+        with pytest.raises(hb.EhError):
+            hb.HipModule(dev, blob, "no_such_entry")
+        after()
+
+
 def test_gradients_of_more_vectors_than_a_launch_has_threads(dev, ops):
     """2^32 vectors and more of one gradient (69 GB, of a row that all share): every row has the same."""
     n, v = 262150, 131072
