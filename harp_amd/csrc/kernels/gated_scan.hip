@@ -10,12 +10,6 @@ namespace eh {
 namespace {
 
 constexpr int kSteps = kScanSteps;   // a thread's own steps, held in registers from the only reading
-constexpr int kLanes = kScanLanes;   // lanes side by side: 128 bytes of a step, a whole cache line
-
-template <int DT> struct Chunk {
-  static constexpr int N = Elem<DT>::N;
-  static constexpr int CW = kLanes * N;                                  // channels of a workgroup
-};
 
 // Where a workgroup leaves what later pieces of the same channels need: 64-bit words (A, B) of its own
 // steps, then 32-bit words of the state behind them.  A word says by itself that it is there: nothing
@@ -153,9 +147,9 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
   }
 }
 
-// A workgroup of W waves has CW channels of W * 64 steps, its piece: eight lanes side by side for the
-// channels, eight runs of kSteps steps one after the other in each wave, the waves one after the
-// other.  Gates and inputs are read once and stay in registers.  Each thread's map, then scans over the
+// A workgroup of W waves has CW channels of W * 512 / LANES steps, its piece: LANES lanes side by side for the
+// channels (eight: 128 bytes of a step, a whole cache line), 64 / LANES runs of kSteps steps one after the other in
+// each wave, the waves one after the other.  Gates and inputs are read once and stay in registers.  Each thread's map, then scans over the
 // lanes, the waves and the pieces of the same channels give the state before each thread's steps, and
 // the steps are run from there.
 //
@@ -179,11 +173,10 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 //
 // Bound by memory: 8 x 4096 x 2048 bf16 at 4.6 TB/s forward and 4.9 backward, 1 x 131072 x 512 f32 at 5.4.  Smaller
 // pieces read the same at more waits and shares of the board, two vectors a lane do not fit the registers.
-// a wave has 64 steps, which the plan's choice of waves goes by, and a workgroup a thread per channel
-static_assert(64 / kLanes * kSteps == 64 && kLanes * 8 <= 64);
-template <int DT, int W, bool BACK, bool LOG, bool FAR, int EU>
+template <int DT, int LANES, int W, bool BACK, bool LOG, bool FAR, int EU>
 __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces, int tiles, int classes, Board board) {
-  constexpr int N = Elem<DT>::N, CW = Chunk<DT>::CW, RUN = W * 64 / kLanes * kSteps, P = 64 * W / CW;
+  constexpr int N = Elem<DT>::N, CW = LANES * N, RUN = W * 64 / LANES * kSteps, P = 64 * W / CW;
+  static_assert(64 % LANES == 0 && CW <= 64 * W, "a thread for each channel of the workgroup");
   typedef typename Elem<DT>::T T;
   __shared__ float maps[2][W][CW];
   __shared__ float others[2][P][CW];
@@ -218,20 +211,21 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
   if (BACK) k = pieces - 1 - k;
   const int64_t b = column / tiles;
   const int tile = static_cast<int>(column % tiles) * CW;
-  const int c0 = tile + (lane % kLanes) * N;
+  const int c0 = tile + (lane % LANES) * N;
   const int nc = a.width - c0;                                            // channels of this thread (above N: N; below 1: none)
   int64_t n = a.time;
   if (a.lengths) n = min(n, max(static_cast<int64_t>(a.lengths[b]), int64_t{0}));
   const int64_t last = n > 0 ? (n - 1) / RUN : 0;                         // the sequence's last piece
   if (k > last) return;
   const int64_t behind = BACK ? last - k : k;                             // pieces before this one, in the order of the steps
-  const int run = wave * (64 / kLanes) + lane / kLanes;                   // this thread's place among the runs
+  const int run = wave * (64 / LANES) + lane / LANES;                   // this thread's place among the runs
   // counted from the piece's first row: this thread's first row, and how many rows the sequence has from there on
-  const int row = (BACK ? W * (64 / kLanes) - 1 - run : run) * kSteps, rows = static_cast<int>(min(n - k * RUN, int64_t{RUN}));
-  const uint32_t cb = static_cast<uint32_t>((lane % kLanes) * N * sizeof(T));
+  const int row = (BACK ? W * (64 / LANES) - 1 - run : run) * kSteps, rows = static_cast<int>(min(n - k * RUN, int64_t{RUN}));
+  const uint32_t cb = static_cast<uint32_t>((lane % LANES) * N * sizeof(T));
 
   u32x4 vg[kSteps] = {}, vx[kSteps] = {};
-  if (n > 0 && nc > 0) {
+  const bool live = nc > 0 && row < rows;                                 // (runs behind a sequence's end load nothing)
+  if (live) {
     load_steps<DT, FAR>({a.gate, b, k * RUN, tile}, row, rows - 1, cb, nc, a.width, vg);
     load_steps<DT, FAR>({BACK ? a.out : a.x, b, k * RUN, tile}, row, rows - 1, cb, nc, a.width, vx);
   }
@@ -240,7 +234,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
   u32x4 vh[BACK ? kSteps : 1];
   auto load_states = [&] {
     const int first = k > 0 ? 1 : 0;
-    if (n > 0 && nc > 0) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, a.width, vh);
+    if (live) load_steps<DT, FAR>({a.x, b, k * RUN - first, tile}, row - 1 + first, rows - 2 + first, cb, nc, a.width, vh);
   };
   if constexpr (BACK && EU == 2) load_states();
   float A[N], B[N];
@@ -262,7 +256,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
   for (int i = 0; i < kSteps; ++i)
     asm volatile("" : "+v"(vg[i]), "+v"(vx[i]));
 #pragma unroll
-  for (int off = kLanes; off < 64; off *= 2) {
+  for (int off = LANES; off < 64; off *= 2) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float pa = __shfl_up(A[j], off), pb = __shfl_up(B[j], off);
@@ -272,19 +266,19 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
       }
     }
   }
-  if (lane >= 64 - kLanes) {
+  if (lane >= 64 - LANES) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      maps[0][wave][(lane % kLanes) * N + j] = A[j];
-      maps[1][wave][(lane % kLanes) * N + j] = B[j];
+      maps[0][wave][(lane % LANES) * N + j] = A[j];
+      maps[1][wave][(lane % LANES) * N + j] = B[j];
     }
   }
   // the map of the runs before this thread's, in its wave
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const float pa = __shfl_up(A[j], kLanes), pb = __shfl_up(B[j], kLanes);
-    A[j] = lane < kLanes ? 1.f : pa;
-    B[j] = lane < kLanes ? 0.f : pb;
+    const float pa = __shfl_up(A[j], LANES), pb = __shfl_up(B[j], LANES);
+    A[j] = lane < LANES ? 1.f : pa;
+    B[j] = lane < LANES ? 0.f : pb;
   }
   __syncthreads();
 
@@ -336,10 +330,10 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
   if (nc <= 0) return;
   float h[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) h[j] = before[(lane % kLanes) * N + j];
+  for (int j = 0; j < N; ++j) h[j] = before[(lane % LANES) * N + j];
   for (int w = 0; w < wave; ++w)
 #pragma unroll
-    for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(maps[0][w][(lane % kLanes) * N + j], h[j], maps[1][w][(lane % kLanes) * N + j]);
+    for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(maps[0][w][(lane % LANES) * N + j], h[j], maps[1][w][(lane % LANES) * N + j]);
 #pragma unroll
   for (int j = 0; j < N; ++j) h[j] = __builtin_fmaf(A[j], h[j], B[j]);
 
@@ -481,6 +475,8 @@ template <class F> hipError_t by_type(int dtype, F&& f) {
   }
 }
 
+template <int N> using Int = std::integral_constant<int, N>;
+
 template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
   const ScanPlan p = plan_scan(a);
   if (p.waves == 0) {
@@ -491,8 +487,8 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
         return a.log_gate ? queue(scan_short<dt.value, steps.value, BACK, true>, grid, 256, 0, stream, a, vectors)
                           : queue(scan_short<dt.value, steps.value, BACK, false>, grid, 256, 0, stream, a, vectors);
       };
-      if (a.time <= 1) return go(std::integral_constant<int, 1>{});
-      return go(std::integral_constant<int, kSteps>{});
+      if (a.time <= 1) return go(Int<1>{});
+      return go(Int<kSteps>{});
     });
   }
   Board board{};
@@ -506,19 +502,22 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
   }
   const unsigned grid = static_cast<unsigned>(a.batch * p.tiles * p.pieces);
   return by_type(a.dtype, [&](auto dt) {
-    auto go = [&](auto waves, auto is_far, auto eu) {
+    auto go = [&](auto lanes, auto waves, auto is_far, auto eu) {
       const int pieces = static_cast<int>(p.pieces), tiles = static_cast<int>(p.tiles);
-      return a.log_gate ? queue(scan_pieces<dt.value, waves.value, BACK, true, is_far.value, eu.value>, grid, 64 * waves.value, 0, stream, a, pieces, tiles, p.classes, board)
-                        : queue(scan_pieces<dt.value, waves.value, BACK, false, is_far.value, eu.value>, grid, 64 * waves.value, 0, stream, a, pieces, tiles, p.classes, board);
+      return a.log_gate ? queue(scan_pieces<dt.value, lanes.value, waves.value, BACK, true, is_far.value, eu.value>, grid, 64 * waves.value, 0, stream, a, pieces, tiles, p.classes, board)
+                        : queue(scan_pieces<dt.value, lanes.value, waves.value, BACK, false, is_far.value, eu.value>, grid, 64 * waves.value, 0, stream, a, pieces, tiles, p.classes, board);
     };
-    const std::integral_constant<int, 2> two;
-    if (p.far) return go(std::integral_constant<int, 8>{}, std::true_type{}, two);
-    if (p.waves == 1) return go(std::integral_constant<int, 1>{}, std::false_type{}, two);
-    if (p.waves == 4) return go(std::integral_constant<int, 4>{}, std::false_type{}, two);
+    const std::false_type near;
+    if (p.far) return go(Int<8>{}, Int<8>{}, std::true_type{}, Int<2>{});
+    if (p.lanes == 2) return p.waves == 1 ? go(Int<2>{}, Int<1>{}, near, Int<2>{}) : go(Int<2>{}, Int<8>{}, near, Int<4>{});
+    if (p.lanes == 4) return p.waves == 1 ? go(Int<4>{}, Int<1>{}, near, Int<2>{}) : go(Int<4>{}, Int<8>{}, near, Int<4>{});
+    if (p.waves == 1) return go(Int<8>{}, Int<1>{}, near, Int<2>{});
+    if (p.waves == 2) return go(Int<8>{}, Int<2>{}, near, Int<2>{});
+    if (p.waves == 4) return go(Int<8>{}, Int<4>{}, near, Int<2>{});
     if constexpr (BACK && dt.value != kF32) {
-      if (p.wide) return go(std::integral_constant<int, 8>{}, std::false_type{}, two);
+      if (p.wide) return go(Int<8>{}, Int<8>{}, near, Int<2>{});
     }
-    return go(std::integral_constant<int, 8>{}, std::false_type{}, std::integral_constant<int, 4>{});
+    return go(Int<8>{}, Int<8>{}, near, Int<4>{});
   });
 }
 

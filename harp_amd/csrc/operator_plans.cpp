@@ -71,11 +71,15 @@ ScanPlan plan_scan(const ScanArgs& a) {
   ScanPlan p{};
   int64_t step = 0;
   for (int64_t s : {a.gate.step, a.x.step, a.out.step, a.grad_gate.step, a.grad_x.step}) step = std::max(step, s);
-  p.far = step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 + 1) >= (int64_t{1} << 32);
   const int64_t vectors = (a.width * static_cast<int64_t>(elem_size(a.dtype)) + 15) / 16;
-  p.waves = a.time <= kScanSteps || (a.time <= 3 * kScanSteps && a.batch * vectors >= (1 << 16)) ? 0 : p.far ? 8 : a.time <= 64 ? 1 : a.time <= 256 ? 4 : 8;
-  const int64_t piece = std::max(p.waves, 1) * (64 / kScanLanes) * kScanSteps;
-  p.channels = kScanLanes * (16 / static_cast<int>(elem_size(a.dtype)));
+  p.lanes = vectors <= 2 ? 2 : vectors <= 4 ? 4 : 8;
+  // a piece's rows and the one before them
+  p.far = step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 / p.lanes * kScanSteps + 1) >= (int64_t{1} << 32);
+  if (p.far) p.lanes = 8;
+  const int64_t wave = 64 / p.lanes * kScanSteps;
+  p.waves = a.time <= kScanSteps || (a.time <= 3 * kScanSteps && a.batch * vectors >= (1 << 16)) ? 0 : p.far ? 8 : a.time <= wave ? 1 : p.lanes < 8 ? 8 : a.time <= 2 * wave ? 2 : a.time <= 4 * wave ? 4 : 8;
+  const int64_t piece = std::max(p.waves, 1) * wave;
+  p.channels = p.lanes * (16 / static_cast<int>(elem_size(a.dtype)));
   p.pieces = std::max<int64_t>((a.time + piece - 1) / piece, 1);
   p.tiles = (a.width + p.channels - 1) / p.channels;
   p.per_group = std::max(64 * p.waves / p.channels, 1);

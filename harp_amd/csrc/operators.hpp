@@ -126,10 +126,10 @@ struct ScanArgs {
   int compute_units;
   void* workspace;
 };
-// A workgroup of `waves` waves has kScanLanes vectors of channels and a piece of waves * 64 steps.
+// A workgroup of `waves` waves has `lanes` vectors of channels and a piece of waves * 64 / lanes * kScanSteps steps.
 constexpr int kScanSteps = 8;        // of a thread
-constexpr int kScanLanes = 8;        // side by side
 struct ScanPlan {
+  int lanes;                         // side by side: 2, 4 or 8
   int waves;                         // 0: a thread has a whole sequence's steps of its channels
   bool far;                          // a piece's rows may lie further apart than 32-bit offsets reach
   int channels;                      // of a workgroup

@@ -380,9 +380,9 @@ static void recurrences(eh_device* d) {
   a.out.offset = 38;
   CHECK(eh_gated_scan(d, &a, 0) != EH_OK);
   eh_gated_scan_backward_args b{};
-  b.batch = 3, b.time = 700, b.width = 10;
-  b.gate = p.array(3, 700, 10, EH_F32), b.h = p.array(3, 700, 10, EH_F32), b.grad_h = p.array(3, 700, 10, EH_F32);
-  b.grad_gate = p.array(3, 700, 10, EH_F32), b.grad_x = p.array(3, 700, 10, EH_F32);
+  b.batch = 3, b.time = 1100, b.width = 10;
+  b.gate = p.array(3, 1100, 10, EH_F32), b.h = p.array(3, 1100, 10, EH_F32), b.grad_h = p.array(3, 1100, 10, EH_F32);
+  b.grad_gate = p.array(3, 1100, 10, EH_F32), b.grad_x = p.array(3, 1100, 10, EH_F32);
   CHECK(eh_gated_scan_backward(d, &b, 0) == EH_OK);
   b.state = p.array(3, 1, 10, EH_F32), b.grad_state = p.array(3, 1, 10, EH_F32), b.grad_final = p.array(3, 1, 10, EH_F32);
   CHECK(eh_gated_scan_backward(d, &b, 0) == EH_OK);
@@ -422,10 +422,11 @@ static void plans() {
     a.dtype = dtype, a.batch = next(1, 1 << 16), a.time = next(1, int64_t{1} << 31), a.width = static_cast<int>(next(1, 1 << 18));
     a.gate.step = a.x.step = a.out.step = next(1, int64_t{1} << 40);
     const ScanPlan p = plan_scan(a);
-    ok = ok && (p.waves == 0 || p.waves == 1 || p.waves == 4 || p.waves == 8) && (p.classes == 1 || p.classes == 8);
-    ok = ok && (p.waves == 0 || (p.pieces * p.waves * 64 >= a.time && (p.pieces - 1) * p.waves * 64 < a.time));
+    const int64_t wave = 64 / p.lanes * kScanSteps;
+    ok = ok && (p.lanes == 2 || p.lanes == 4 || p.lanes == 8) && (p.waves == 0 || p.waves == 1 || p.waves == 8 || (p.lanes == 8 && (p.waves == 2 || p.waves == 4))) && (p.classes == 1 || p.classes == 8);
+    ok = ok && (p.waves == 0 || (p.pieces * p.waves * wave >= a.time && (p.pieces - 1) * p.waves * wave < a.time));
     ok = ok && (p.pieces == 1 || p.waves == 8 || (p.waves == 0 && a.time <= 3 * kScanSteps)) && p.tiles * p.channels >= a.width && (p.tiles - 1) * p.channels < a.width;
-    ok = ok && (p.far || a.gate.step * static_cast<int64_t>(elem_size(dtype)) * (p.waves * 64 + 1) < (int64_t{1} << 32));
+    ok = ok && (p.far || a.gate.step * static_cast<int64_t>(elem_size(dtype)) * (p.waves * wave + 1) < (int64_t{1} << 32)) && (!p.far || (p.lanes == 8 && (p.waves == 8 || p.waves == 0)));
     ok = ok && p.groups * p.per_group >= p.pieces && (p.waves != 8 || p.per_group * p.channels == 512);
     ++g_checks;
     if (!ok) {

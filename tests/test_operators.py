@@ -403,6 +403,15 @@ def test_scan_last_channels(dev, ops, dtype, log_gate):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("width", [1, 8, 9, 16, 17, 31])
+def test_scan_of_few_channels(dev, ops, width, dtype):
+    """Rows of less than a cache line: more steps go to a workgroup, in one piece and in several."""
+    check_scan(dev, ops, 9, 130, width, dtype, log_gate=True)
+    check_scan(dev, ops, 2, 4300, width, dtype, log_gate=False, lengths=[4300, 2049])
+    check_scan(dev, ops, 3, 1100, width, dtype, log_gate=True, layout="wide", state=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_scan_lengths(dev, ops, dtype):
     """Sequences of no steps, one, all, and lengths outside the array; NaN behind them stays there."""
     check_scan(dev, ops, 7, 150, 48, dtype, log_gate=True, lengths=[0, 1, 150, 149, -3, 1000, 64])
