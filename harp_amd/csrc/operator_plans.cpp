@@ -82,7 +82,7 @@ ScanPlan plan_scan(const ScanArgs& a) {
   p.channels = p.lanes * (16 / static_cast<int>(elem_size(a.dtype)));
   p.pieces = std::max<int64_t>((a.time + piece - 1) / piece, 1);
   p.tiles = (a.width + p.channels - 1) / p.channels;
-  p.per_group = std::max(64 * p.waves / p.channels, 1);
+  p.per_group = p.waves == 8 ? 128 / p.lanes : 1;                       // 512 threads read one word each in f32, two in 16 bits
   p.groups = (p.pieces + p.per_group - 1) / p.per_group;
   bool lines = true;
   for (const Sequences* s : {&a.gate, &a.x, &a.out, &a.grad_gate, &a.grad_x})

@@ -427,7 +427,7 @@ static void plans() {
     ok = ok && (p.waves == 0 || (p.pieces * p.waves * wave >= a.time && (p.pieces - 1) * p.waves * wave < a.time));
     ok = ok && (p.pieces == 1 || p.waves == 8 || (p.waves == 0 && a.time <= 3 * kScanSteps)) && p.tiles * p.channels >= a.width && (p.tiles - 1) * p.channels < a.width;
     ok = ok && (p.far || a.gate.step * static_cast<int64_t>(elem_size(dtype)) * (p.waves * wave + 1) < (int64_t{1} << 32)) && (!p.far || (p.lanes == 8 && (p.waves == 8 || p.waves == 0)));
-    ok = ok && p.groups * p.per_group >= p.pieces && (p.waves != 8 || p.per_group * p.channels == 512);
+    ok = ok && p.groups * p.per_group >= p.pieces && (p.waves != 8 || p.per_group * p.lanes == 128);
     ++g_checks;
     if (!ok) {
       ++g_failures;
