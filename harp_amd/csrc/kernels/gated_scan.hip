@@ -150,16 +150,16 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 // A workgroup of W waves has CW channels of W * 512 / LANES steps, its piece: LANES lanes side by side for the
 // channels (eight: 128 bytes of a step, a whole cache line), 64 / LANES runs of kSteps steps one after the other in
 // each wave, the waves one after the other.  (With eight lanes for rows of fewer vectors most would be idle:
-// 256 x 20000 x 9 bf16 278 us instead of 118, 16 x 131072 x 8 f16 96 instead of 38.)  Gates and inputs are read once and stay in registers.  Each thread's map, then scans over the
-// lanes, the waves and the pieces of the same channels give the state before each thread's steps, and
-// the steps are run from there.
+// 256 x 20000 x 9 bf16 278 us instead of 118, 16 x 131072 x 8 f16 96 instead of 38.)  Gates and inputs are read
+// once and stay in registers.  Each thread's map, then scans over the lanes, the waves and the pieces of the same
+// channels give the state before each thread's steps, and the steps are run from there.
 //
 // Over the pieces (W == 8; shorter sequences have one): they form groups of P in the order of the
 // steps.  Each leaves its map on the board before it looks at anybody else's, the last of a group the
 // state behind it; a piece composes the state before its group with the maps of the group's pieces
 // before it, all read at once (128 / LANES pieces: one word a thread in f32, two in 16 bits, where with one
-// the wait from group to group made 1 x 131072 x 64 bf16 40 us instead of 29).  Which words are read depends on the piece alone, so results do not
-// depend on the order in which workgroups run.
+// the wait from group to group made 1 x 131072 x 64 bf16 40 us instead of 29).  Which words are read depends on
+// the piece alone, so results do not depend on the order in which workgroups run.
 //
 // Columns (a sequence's channels of one workgroup's width) are dealt to classes in runs of neighbours;
 // a workgroup takes a ticket of its class, of the next one where that has no pieces left.  A class's

@@ -484,6 +484,7 @@ struct Teacher {
   __device__ Teacher(float* lds, int k)
       : ids(reinterpret_cast<int*>(lds)), next(ids + k), q(lds + 2 * k), log_q(lds + 3 * k), sum(lds + 4 * k), z(lds + 5 * k),
         head(ids + 6 * k) {}
+  __host__ __device__ static size_t bytes16(int k, int threads) { return (24 * static_cast<size_t>(k) + 4 * static_cast<size_t>(threads) + 15) / 16 * 16; }
   static size_t bytes(int k, int threads) { return 24 * static_cast<size_t>(k) + 4 * static_cast<size_t>(threads); }
 };
 extern __shared__ float teacher_lds[];
@@ -598,7 +599,9 @@ __device__ inline void write_named(const Teacher& t, const Gradient& g, typename
 // row of 250 KB on a compute unit by the waits between its reading and its writing too: 8192 x 128000
 // bf16 in 829 us (5.1 TB/s).  Read a second time instead: 1280 us with four times as many rows on the
 // way as the last-level cache holds, 950 us with as many as it does hold.
-template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillArgs a) {
+// EX: vectors a thread keeps in LDS besides, read first, while the registers are free (3000 x 80000 f32 376 us;
+// with two readings, the loss and then the gradient from what it leaves, 480).
+template <int DT, int THREADS, int NV, int EX> __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillArgs a) {
   constexpr int N = Elem<DT>::N;
   typedef typename Elem<DT>::T T;
   __shared__ float lds[2 * THREADS / 64];
@@ -608,11 +611,25 @@ template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) 
   const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride;
   T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
   const Entry first(a, row, threadIdx.x);
+  const u32x4 nothing = {Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity};
+  u32x4* kept = reinterpret_cast<u32x4*>(reinterpret_cast<char*>(teacher_lds) + Teacher::bytes16(a.k, THREADS)) + threadIdx.x;
+  if constexpr (EX > 0) {
+    u32x4 v[EX];
+#pragma unroll
+    for (int i = 0; i < EX; ++i) {
+      const int at = (NV + i) * THREADS + static_cast<int>(threadIdx.x);
+      v[i] = nothing;
+      if (at < full) v[i] = load16(p + at * N);
+    }
+#pragma unroll
+    for (int i = 0; i < EX; ++i) kept[i * THREADS] = v[i];
+    __builtin_amdgcn_sched_barrier(0);                      // the other loads need these registers
+  }
   u32x4 v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int at = i * THREADS + static_cast<int>(threadIdx.x);
-    v[i] = u32x4{Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity, Elem<DT>::kMinusInfinity};
+    v[i] = nothing;
     if (at < full) v[i] = load16(p + at * N);
   }
   const bool tail = static_cast<int>(threadIdx.x) < rest;
@@ -629,6 +646,13 @@ template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) 
     Elem<DT>::unpack(v[i + 1], z + N);
     add_elements<2 * N, false>(mine, z, c2);
   }
+#pragma unroll 1
+  for (int i = 0; i < EX; i += 2) {
+    float z[2 * N];
+    Elem<DT>::unpack(kept[i * THREADS], z);
+    Elem<DT>::unpack(kept[(i + 1) * THREADS], z + N);
+    add_elements<2 * N, false>(mine, z, c2);
+  }
   const float z[4] = {last, -INFINITY, -INFINITY, -INFINITY};
   add_elements<4, false>(mine, z, c2);
   const RowSums r = join_and_report<DT, THREADS>(a, row, mine, zk, total, teacher, lds);
@@ -642,6 +666,16 @@ template <int DT, int THREADS, int NV> __global__ __launch_bounds__(THREADS, 4) 
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
     if (at < full) store16(out + at * N, Elem<DT>::pack(z));
+  }
+#pragma unroll 1
+  for (int i = 0; i < EX; ++i) {
+    const int at = (NV + i) * THREADS + static_cast<int>(threadIdx.x);
+    if (at >= full) break;
+    float z[N];
+    Elem<DT>::unpack(kept[i * THREADS], z);
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
+    store16(out + at * N, Elem<DT>::pack(z));
   }
   if (tail) out[full * N + threadIdx.x] = Elem<DT>::put(gradient(last));
   write_named<DT>(teacher, gradient, out);
@@ -697,42 +731,16 @@ template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distil
       out[id] = Elem<DT>::put(gradient(k < THREADS ? zk : student<DT>(a, row, id)) - gradient.w * teacher.sum[k]);
 }
 
-// The loss alone, or (GRAD) rows longer than a workgroup's registers hold: a second reading.
-template <int DT, int THREADS, bool GRAD> __global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
-  constexpr int N = Elem<DT>::N, U = 4;
-  typedef typename Elem<DT>::T T;
+// The loss alone.
+template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distill_rows(DistillArgs a) {
   __shared__ float lds[2 * THREADS / 64];
   const Teacher teacher(teacher_lds, a.k);
   const int64_t row = blockIdx.x;
-  const int n = a.in.vocab;
-  const T* p = static_cast<const T*>(a.in.z) + row * a.in.stride;
+  const Segment<DT> part(static_cast<const typename Elem<DT>::T*>(a.in.z) + row * a.in.stride, a.in.vocab);
   const Entry first(a, row, threadIdx.x);
   const float zk = student<DT>(a, row, first.id);
-  const float total = load_teacher<THREADS, N, GRAD>(a, row, first, teacher, lds);
-  const RowSums r = join_and_report<DT, THREADS>(a, row, sum_row<DT, THREADS, false>(Segment<DT>(p, n), a.in.scale * kLog2e), zk, total, teacher, lds);
-  if constexpr (GRAD) {
-    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
-    const Gradient gradient(a, row, r.m, log2_hw(r.s), r.s == 0.f, total);
-    const int full = n / N;
-    for (int i = threadIdx.x; i < full; i += U * THREADS) {
-      u32x4 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * THREADS < full) v[u] = load16(p + static_cast<int64_t>(i + u * THREADS) * N);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u * THREADS >= full) break;
-        float z[N];
-        Elem<DT>::unpack(v[u], z);
-#pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
-        store16(out + static_cast<int64_t>(i + u * THREADS) * N, Elem<DT>::pack(z));
-      }
-    }
-    const int at = full * N + static_cast<int>(threadIdx.x);
-    if (at < n) out[at] = Elem<DT>::put(gradient(Elem<DT>::get(p[at])));
-    write_named<DT>(teacher, gradient, out);
-  }
+  const float total = load_teacher<THREADS, Elem<DT>::N, false>(a, row, first, teacher, lds);
+  join_and_report<DT, THREADS>(a, row, sum_row<DT, THREADS, false>(part, a.in.scale * kLog2e), zk, total, teacher, lds);
 }
 
 // Few rows that are long: segments' sums, then a workgroup a row joins them and finds the loss.
@@ -780,6 +788,7 @@ template <class F> hipError_t by_items(int items, F&& f) {
     default: return f(std::integral_constant<int, kScoreHeld>{});
   }
 }
+template <int N> using Int = std::integral_constant<int, N>;
 unsigned grid_of(int64_t n) { return static_cast<unsigned>(n); }
 // `spans` workgroups for each row, in launches of as many rows as one can have.
 template <class F> hipError_t by_row_runs(int64_t rows, int spans, F&& f) {
@@ -850,28 +859,29 @@ hipError_t launch_distill(const DistillArgs& a, hipStream_t stream) {
       const hipError_t e = queue(distill_join<DT, 256>, rows, 256, Teacher::bytes(a.k, 256), stream, a);
       return e != hipSuccess || !a.grad ? e : launch_gradient_alone<DT>(a, stream);
     }
-    if (!a.grad)
-      return by_threads(a.split.threads, [&](auto threads) {
-        return queue(distill_rows<DT, threads.value, false>, rows, threads.value, Teacher::bytes(a.k, threads.value), stream, a);
+    if (!a.grad || a.held.vectors == 0) {
+      const hipError_t e = by_threads(a.split.threads, [&](auto threads) {
+        return queue(distill_rows<DT, threads.value>, rows, threads.value, Teacher::bytes(a.k, threads.value), stream, a);
       });
+      return e != hipSuccess || !a.grad ? e : launch_gradient_alone<DT>(a, stream);
+    }
     auto held = [&](auto threads, auto nv) {
-      return queue(distill_held<DT, threads.value, nv.value>, rows, threads.value, Teacher::bytes(a.k, threads.value), stream, a);
+      return queue(distill_held<DT, threads.value, nv.value, 0>, rows, threads.value, Teacher::bytes(a.k, threads.value), stream, a);
     };
-    const std::integral_constant<int, 4> four;
-    const std::integral_constant<int, 16> sixteen;
-    const std::integral_constant<int, 256> t256;
-    const std::integral_constant<int, 1024> t1024;
-    if (a.held.vectors == 4) {
-      if (a.held.threads == 64) return held(std::integral_constant<int, 64>{}, four);
-      if (a.held.threads == 256) return held(t256, four);
-      return held(t1024, four);
+    const RowHeld h = a.held;
+    if (h.vectors == 4) {
+      if (h.threads == 64) return held(Int<64>{}, Int<4>{});
+      if (h.threads == 128) return held(Int<128>{}, Int<4>{});
+      if (h.threads == 256) return held(Int<256>{}, Int<4>{});
+      return held(Int<1024>{}, Int<4>{});
     }
-    if (a.held.vectors == 16) {
-      if (a.held.threads == 256) return held(t256, sixteen);
-      if (a.held.threads == 512) return held(std::integral_constant<int, 512>{}, sixteen);
-      return held(t1024, sixteen);
+    if (h.vectors == 8) return held(Int<256>{}, Int<8>{});
+    if (h.vectors == 16) {
+      if (h.threads == 256) return held(Int<256>{}, Int<16>{});
+      if (h.threads == 512) return held(Int<512>{}, Int<16>{});
+      return held(Int<1024>{}, Int<16>{});
     }
-    return queue(distill_rows<DT, 1024, true>, rows, 1024, Teacher::bytes(a.k, 1024), stream, a);
+    return queue(distill_held<DT, 1024, 16, kHeldInLds>, rows, 1024, Teacher::bytes16(a.k, 1024) + 16 * 1024 * kHeldInLds, stream, a);
   });
 }
 

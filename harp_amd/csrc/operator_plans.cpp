@@ -44,14 +44,19 @@ size_t split_workspace(const RowSplit& s, int64_t rows, int top) {
 // The smallest workgroup that holds a row, with few rows the largest (us a call):
 //   16384 x 1000 bf16     64 x 4 20.9, 256 x 4 49         4096 x 64000 bf16   512 x 16 204, 1024 x 16 245
 //   4096 x 32000 bf16    256 x 16 108, 1024 x 16 156      256 x 32000 bf16    1024 x 4 11.9, 256 x 16 13.8
+//   16384 x 4000 bf16    128 x 4 49, 256 x 4 59           8192 x 12000 bf16   256 x 8 78, 256 x 16 88 (8192 x 8000 f32 103, 97)
+//   8192 x 190000 bf16   1024 x (16 + 8 in LDS) 1278, in two readings 1546, as rows that are longer still are taken
 RowHeld hold_rows(int64_t rows, int vocab, int dtype, int compute_units) {
   const int64_t vectors = vocab / (16 / static_cast<int64_t>(elem_size(dtype)));
   if (vectors <= 256) return {64, 4};
   if (rows <= 2 * static_cast<int64_t>(compute_units) && vectors <= 4096) return {1024, 4};
+  if (vectors <= 512) return {128, 4};
   if (vectors <= 1024) return {256, 4};
+  if (vectors <= 2048 && dtype != kF32) return {256, 8};
   if (vectors <= 4096) return {256, 16};
   if (vectors <= 8192) return {512, 16};
   if (vectors <= 16384) return {1024, 16};
+  if (vectors <= 1024 * (16 + kHeldInLds)) return {1024, 16 + kHeldInLds};
   return {1024, 0};
 }
 

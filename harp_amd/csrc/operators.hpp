@@ -51,6 +51,7 @@ struct RowPartial {
 size_t split_workspace(const RowSplit& s, int64_t rows, int top);   // bytes; 0 for whole rows
 
 // A row held in a workgroup's registers, `vectors` of 16 bytes a thread; 0 vectors: too long for that.
+constexpr int kHeldInLds = 8;        // vectors of a thread in LDS besides 16 in registers, of the longest rows
 struct RowHeld {
   int threads;
   int vectors;

@@ -416,7 +416,8 @@ static void plans() {
     ok = ok && (!r.held || (!top && r.segs == 1 && held_form(r.threads, r.held) && static_cast<int64_t>(r.threads) * r.held * vec >= static_cast<int64_t>(vocab) + vec - 1));
     const RowHeld h = hold_rows(rows, vocab, dtype, 256);
     ok = ok && (h.vectors == 0 || static_cast<int64_t>(h.threads) * h.vectors >= vocab / vec);
-    ok = ok && (h.vectors == 0 || (h.vectors == 4 && (h.threads == 64 || h.threads == 256 || h.threads == 1024)) ||
+    ok = ok && (h.vectors == 0 || (h.vectors == 4 && (h.threads == 64 || h.threads == 128 || h.threads == 256 || h.threads == 1024)) ||
+                (h.vectors == 8 && h.threads == 256) || (h.vectors == 24 && h.threads == 1024) ||
                 (h.vectors == 16 && (h.threads == 256 || h.threads == 512 || h.threads == 1024)));
     ScanArgs a{};
     a.dtype = dtype, a.batch = next(1, 1 << 16), a.time = next(1, int64_t{1} << 31), a.width = static_cast<int>(next(1, 1 << 18));

@@ -250,7 +250,8 @@ def check_distill(dev, ops, z, u, ids, temperature, weight, dtype, workspace=Non
 
 DISTILL = [(1, 1, 1), (1, 5, 3), (3, 64, 7), (2, 1000, 100), (6, 2051, 1), (1, 50000, 40), (9, 9000, 257), (3, 1100, 1024), (1030, 97, 5)]
 DISTILL_SHAPES = [("f32", 3, 16001, 30), ("f32", 520, 4001, 3), ("bf16", 520, 16003, 70), ("f32", 520, 32001, 5), ("f32", 3, 60001, 1024), ("bf16", 2, 131075, 65),
-                  ("f32", 70, 70001, 20), ("f16", 2, 140003, 200), ("f32", 2, 140001, 20), ("bf16", 1, 300000, 300)]
+                  ("f32", 70, 70001, 20), ("f16", 2, 140003, 200), ("f32", 2, 140001, 20), ("bf16", 1, 300000, 300),
+                  ("f16", 520, 1003, 8), ("bf16", 520, 3001, 9), ("f32", 520, 7001, 4), ("f16", 3, 196613, 1024), ("f32", 3, 98304, 9), ("f32", 70, 98410, 5), ("bf16", 2, 131079, 3)]
 
 
 @pytest.mark.parametrize("dtype,n,v,k", DISTILL_SHAPES)
