@@ -498,7 +498,7 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
   }
   Board board{};
   if (p.pieces > 1) {
-    const size_t words = scan_workspace(a) / 4;
+    const size_t words = scan_board(a, p) / 4;
     board.tickets = static_cast<unsigned int*>(a.workspace);
     board.maps = reinterpret_cast<unsigned long long*>(board.tickets + kTicketBytes / 4);
     board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.pieces * p.channels);

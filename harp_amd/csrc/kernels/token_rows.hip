@@ -822,7 +822,10 @@ hipError_t launch_score(const ScoreArgs& a, hipStream_t stream) {
           });
         }
       }
-      return queue(score_rows<dt.value, threads.value, ent.value, top.value>, grid_of(a.in.rows * a.split.segs), threads.value, 0, stream, a);
+      // (shorter rows without alternatives are held)
+      if constexpr (top.value || threads.value >= 256)
+        return queue(score_rows<dt.value, threads.value, ent.value, top.value>, grid_of(a.in.rows * a.split.segs), threads.value, 0, stream, a);
+      else return hipErrorInvalidValue;
     });
     if (e != hipSuccess || a.split.segs == 1) return e;
     return queue(score_join<256, ent.value, top.value>, grid_of(a.in.rows), 256, 0, stream, a);

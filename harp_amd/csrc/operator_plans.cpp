@@ -32,7 +32,7 @@ RowSplit split_rows(int64_t rows, int vocab, int dtype, bool top, int compute_un
   }
   if (rows <= compute_units) return {items <= 256 ? 64 : items <= 512 ? 128 : items <= 1024 ? 256 : items <= 2048 ? 512 : 1024, 0, 1, vocab};
   if (items <= 512) return {64, 0, 1, vocab};
-  if (items <= 2048) return {128, 0, 1, vocab};
+  if (items <= 2048 && top) return {128, 0, 1, vocab};
   return {items > 4096 && rows >= 8 * static_cast<int64_t>(compute_units) ? 512 : 256, 0, 1, vocab};
 }
 
@@ -98,11 +98,16 @@ ScanPlan plan_scan(const ScanArgs& a) {
   return p;
 }
 
-size_t scan_workspace(const ScanArgs& a) {
-  const ScanPlan p = plan_scan(a);
+size_t scan_board(const ScanArgs& a, const ScanPlan& p) {
   if (p.pieces == 1) return 0;
   return kTicketBytes + static_cast<size_t>(a.batch * p.tiles) * static_cast<size_t>(p.channels) *
                             (8 * static_cast<size_t>(p.pieces) + 4 * static_cast<size_t>(p.groups));
+}
+
+size_t scan_workspace(const ScanArgs& a) {
+  ScanArgs apart = a;
+  apart.gate.step = int64_t{1} << 40;
+  return std::max(scan_board(a, plan_scan(a)), scan_board(apart, plan_scan(apart)));
 }
 
 }  // namespace eh

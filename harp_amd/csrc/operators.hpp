@@ -141,7 +141,8 @@ struct ScanPlan {
 };
 ScanPlan plan_scan(const ScanArgs& a);
 constexpr size_t kTicketBytes = 256;
-size_t scan_workspace(const ScanArgs& a);     // bytes; 0 where a sequence is one piece
+size_t scan_board(const ScanArgs& a, const ScanPlan& p);      // bytes; 0 where a sequence is one piece
+size_t scan_workspace(const ScanArgs& a);     // what sequences of these sizes may need, whatever their strides
 hipError_t launch_scan(const ScanArgs& a, hipStream_t stream);
 hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t stream);
 

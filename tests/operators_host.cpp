@@ -424,6 +424,10 @@ static void plans() {
     a.gate.step = a.x.step = a.out.step = next(1, int64_t{1} << 40);
     const ScanPlan p = plan_scan(a);
     const int64_t wave = 64 / p.lanes * kScanSteps;
+    ScanArgs close = a;                          // a workspace is asked for without the arrays' strides
+    close.gate.step = close.x.step = close.out.step = a.width;
+    ok = ok && scan_workspace(close) == scan_workspace(a) && scan_workspace(a) >= scan_board(a, p);
+    ok = ok && (r.segs > 1 || r.held || top || r.threads >= 256);
     ok = ok && (p.lanes == 2 || p.lanes == 4 || p.lanes == 8) && (p.waves == 0 || p.waves == 1 || p.waves == 8 || (p.lanes == 8 && (p.waves == 2 || p.waves == 4))) && (p.classes == 1 || p.classes == 8);
     ok = ok && (p.waves == 0 || (p.pieces * p.waves * wave >= a.time && (p.pieces - 1) * p.waves * wave < a.time));
     ok = ok && (p.pieces == 1 || p.waves == 8 || (p.waves == 0 && a.time <= 3 * kScanSteps)) && p.tiles * p.channels >= a.width && (p.tiles - 1) * p.channels < a.width;

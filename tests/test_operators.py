@@ -706,6 +706,27 @@ def test_gradients_of_more_vectors_than_a_launch_has_threads(dev, ops):
     same(one)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_few_channels_with_steps_far_apart(dev, ops, dtype):
+    """Steps of megabytes, so that a piece reaches beyond 32-bit offsets, in the workspace that was asked for."""
+    t, d, step = 2500, 8, 1_200_000
+    base = torch.zeros(t * step + d, device="cuda", dtype=DT[dtype])
+    gate, x, gh = sequences(1, t, d, dtype, 3, True)
+    far = [base[i * 64:].as_strided((1, t, d), (0, step, 1)) for i in range(6)]
+    for a, b in zip(far, (gate, x, gh)):
+        a.copy_(b)
+    h, gg, gx = far[3:]
+    ws = torch.empty(ops.gated_scan_workspace(dev, gate), device="cuda", dtype=torch.uint8)
+    ops.gated_scan(dev, far[0], far[1], log_gate=True, out=h, workspace=ws)
+    want, tol, _, _ = oracle.scan(host(gate), host(x), None, None, True)
+    close(host(h), want, tol + oracle.rounding(dtype, want), "h")
+    ws = torch.empty(ops.gated_scan_backward_workspace(dev, gate), device="cuda", dtype=torch.uint8)
+    ops.gated_scan_backward(dev, far[0], h, far[2], log_gate=True, out=ops.ScanGrads(gg, gx, None), workspace=ws)
+    want, tols = oracle.scan_grad(host(gate), host(h), host(gh), None, None, True, None)
+    for name, got, w, tl in zip(("grad_gate", "grad_x"), (gg, gx), want, tols):
+        close(host(got), w, tl + oracle.rounding(dtype, w), name)
+
+
 REFUSED = [
     ("overlap", lambda o, d, z, t, e: o.token_logprobs_backward(d, z, t, e(4, 2), out=z)),
     ("overlap", lambda o, d, z, t, e: o.gated_scan(d, z[None], z[None], out=z[None])),
