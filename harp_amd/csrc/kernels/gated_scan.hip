@@ -154,7 +154,7 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 // once and stay in registers.  Each thread's map, then scans over the lanes, the waves and the pieces of the same
 // channels give the state before each thread's steps, and the steps are run from there.
 //
-// Over the pieces (W == 8; shorter sequences have one): they form groups of P in the order of the
+// Over the pieces (W == 8; other sequences have one): they form groups of P in the order of the
 // steps.  Each leaves its map on the board before it looks at anybody else's, the last of a group the
 // state behind it; a piece composes the state before its group with the maps of the group's pieces
 // before it, all read at once (128 / LANES pieces: one word a thread in f32, two in 16 bits, where with one
@@ -519,6 +519,7 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
     if (p.waves == 1) return go(Int<8>{}, Int<1>{}, near, Int<2>{});
     if (p.waves == 2) return go(Int<8>{}, Int<2>{}, near, Int<2>{});
     if (p.waves == 4) return go(Int<8>{}, Int<4>{}, near, Int<2>{});
+    if (p.waves == 16) return go(Int<8>{}, Int<16>{}, near, Int<4>{});
     if constexpr (BACK && dt.value != kF32) {
       if (p.wide) return go(Int<8>{}, Int<8>{}, near, Int<2>{});
     }

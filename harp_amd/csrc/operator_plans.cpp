@@ -68,6 +68,8 @@ static bool on_lines(const Sequences& s, const ScanArgs& a) {
 
 // Sequences of a few steps by a thread each, where that fills the device (1024 x 9 x 2048 bf16 20 us against 69
 // with a piece's 64 steps for each, 64 x 16 x 2048 8 us against 8.5, from 32 steps on no difference).
+// One piece of 16 waves instead of two of 8 with a board: 16 x 700 x 2048 bf16 32 us against 36, 64 x 520 x 1024 57
+// against 64, but many of all 1024 steps 32 x 1000 x 2048 96 against 88 (one workgroup on a compute unit).
 // Wide: one workgroup on a compute unit instead of two, us a gradient with and without, by workgroups of a compute unit:
 //   one    4 x 1999 x 717 f16 19.3 : 20.5       two   4 x 4096 x 1024 bf16 38 : 34, 32 x 512 x 704 f16 27 : 21
 //   eight  8 x 4096 x 2048 bf16 136 : 145       more  64 x 4096 x 1024 bf16 496 : 537, 52 x 2048 x 717 f16 210 : 222
@@ -78,15 +80,24 @@ ScanPlan plan_scan(const ScanArgs& a) {
   for (int64_t s : {a.gate.step, a.x.step, a.out.step, a.grad_gate.step, a.grad_x.step}) step = std::max(step, s);
   const int64_t vectors = (a.width * static_cast<int64_t>(elem_size(a.dtype)) + 15) / 16;
   p.lanes = vectors <= 2 ? 2 : vectors <= 4 ? 4 : 8;
-  // a piece's rows and the one before them
-  p.far = step * static_cast<int64_t>(elem_size(a.dtype)) * (8 * 64 / p.lanes * kScanSteps + 1) >= (int64_t{1} << 32);
-  if (p.far) p.lanes = 8;
   const int64_t wave = 64 / p.lanes * kScanSteps;
-  p.waves = a.time <= kScanSteps || (a.time <= 3 * kScanSteps && a.batch * vectors >= (1 << 16)) ? 0 : p.far ? 8 : a.time <= wave ? 1 : p.lanes < 8 ? 8 : a.time <= 2 * wave ? 2 : a.time <= 4 * wave ? 4 : 8;
-  const int64_t piece = std::max(p.waves, 1) * wave;
+  int64_t piece = wave;
+  if (a.time > kScanSteps && (a.time > 3 * kScanSteps || a.batch * vectors < (1 << 16))) {
+    const int64_t tiles = (vectors + p.lanes - 1) / p.lanes;
+    if (a.time <= wave) p.waves = 1;
+    else if (p.lanes < 8) p.waves = 8;
+    else if (a.time <= 2 * wave) p.waves = 2;
+    else if (a.time <= 4 * wave) p.waves = 4;
+    else if (a.time <= 8 * wave) p.waves = 8;
+    else p.waves = a.time <= 10 * wave || (a.time <= 16 * wave && a.batch * tiles <= 2 * static_cast<int64_t>(a.compute_units)) ? 16 : 8;
+    piece = p.waves * wave;
+    // (the rows of a piece and the one before them)
+    p.far = step * static_cast<int64_t>(elem_size(a.dtype)) * (piece + 1) >= (int64_t{1} << 32);
+    if (p.far) p.lanes = 8, p.waves = 8, piece = 8 * 64;
+  }
   p.channels = p.lanes * (16 / static_cast<int>(elem_size(a.dtype)));
-  p.pieces = std::max<int64_t>((a.time + piece - 1) / piece, 1);
   p.tiles = (a.width + p.channels - 1) / p.channels;
+  p.pieces = std::max<int64_t>((a.time + piece - 1) / piece, 1);
   p.per_group = p.waves == 8 ? 128 / p.lanes : 1;                       // 512 threads read one word each in f32, two in 16 bits
   p.groups = (p.pieces + p.per_group - 1) / p.per_group;
   bool lines = true;

@@ -466,7 +466,7 @@ int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync) {
     s.final_state = arrays.small<float>("final_state", a.final_state, a.batch, a.width, EH_F32, false, true);
     s.lengths = arrays.small<const int>("lengths", a.lengths, a.batch, 1, EH_I32, false, false);
     check_plan(s);
-    Workspace ws(d, arrays, a.workspace, scan_workspace(s));
+    Workspace ws(d, arrays, a.workspace, scan_board(s, plan_scan(s)));
     s.workspace = ws.at();
     arrays.settle();
     if (a.batch) launched(launch_scan(s, d->stream()), "launch of gated_scan");
@@ -495,7 +495,7 @@ int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* ar
     s.final_state = arrays.small<float>("grad_state", a.grad_state, a.batch, a.width, EH_F32, false, true);
     s.lengths = arrays.small<const int>("lengths", a.lengths, a.batch, 1, EH_I32, false, false);
     check_plan(s);
-    Workspace ws(d, arrays, a.workspace, scan_workspace(s));
+    Workspace ws(d, arrays, a.workspace, scan_board(s, plan_scan(s)));
     s.workspace = ws.at();
     arrays.settle();
     if (a.batch) launched(launch_scan_grad(s, d->stream()), "launch of gated_scan_backward");

@@ -420,6 +420,7 @@ static void plans() {
                 (h.vectors == 8 && h.threads == 256) || (h.vectors == 24 && h.threads == 1024) ||
                 (h.vectors == 16 && (h.threads == 256 || h.threads == 512 || h.threads == 1024)));
     ScanArgs a{};
+    a.compute_units = 256;
     a.dtype = dtype, a.batch = next(1, 1 << 16), a.time = next(1, int64_t{1} << 31), a.width = static_cast<int>(next(1, 1 << 18));
     a.gate.step = a.x.step = a.out.step = next(1, int64_t{1} << 40);
     const ScanPlan p = plan_scan(a);
@@ -428,10 +429,10 @@ static void plans() {
     close.gate.step = close.x.step = close.out.step = a.width;
     ok = ok && scan_workspace(close) == scan_workspace(a) && scan_workspace(a) >= scan_board(a, p);
     ok = ok && (r.segs > 1 || r.held || top || r.threads >= 256);
-    ok = ok && (p.lanes == 2 || p.lanes == 4 || p.lanes == 8) && (p.waves == 0 || p.waves == 1 || p.waves == 8 || (p.lanes == 8 && (p.waves == 2 || p.waves == 4))) && (p.classes == 1 || p.classes == 8);
+    ok = ok && (p.lanes == 2 || p.lanes == 4 || p.lanes == 8) && (p.waves == 0 || p.waves == 1 || p.waves == 8 || (p.lanes == 8 && (p.waves == 2 || p.waves == 4 || (p.waves == 16 && p.pieces == 1)))) && (p.classes == 1 || p.classes == 8);
     ok = ok && (p.waves == 0 || (p.pieces * p.waves * wave >= a.time && (p.pieces - 1) * p.waves * wave < a.time));
     ok = ok && (p.pieces == 1 || p.waves == 8 || (p.waves == 0 && a.time <= 3 * kScanSteps)) && p.tiles * p.channels >= a.width && (p.tiles - 1) * p.channels < a.width;
-    ok = ok && (p.far || a.gate.step * static_cast<int64_t>(elem_size(dtype)) * (p.waves * wave + 1) < (int64_t{1} << 32)) && (!p.far || (p.lanes == 8 && (p.waves == 8 || p.waves == 0)));
+    ok = ok && (p.waves == 0 || p.far || a.gate.step * static_cast<int64_t>(elem_size(dtype)) * (p.waves * wave + 1) < (int64_t{1} << 32)) && (!p.far || (p.lanes == 8 && (p.waves == 8 || p.waves == 0)));
     ok = ok && p.groups * p.per_group >= p.pieces && (p.waves != 8 || p.per_group * p.lanes == 128);
     ++g_checks;
     if (!ok) {

@@ -399,6 +399,7 @@ def test_scan_last_channels(dev, ops, dtype, log_gate):
     check_scan(dev, ops, 6, 1030, 717, dtype, log_gate, lengths=[1030, 1, 513, 1029, 700, 1030])
     check_scan(dev, ops, 16, 600, 717, dtype, log_gate)       # (more workgroups than the device runs one a compute unit)
     check_scan(dev, ops, 5, 1100, 1408, dtype, log_gate)
+    check_scan(dev, ops, 2, 1021, 203, dtype, log_gate)
     for width in (65, 74, 83, 92, 102, 111):
         check_scan(dev, ops, 3, 530, width, dtype, log_gate)
 
@@ -709,8 +710,8 @@ def test_gradients_of_more_vectors_than_a_launch_has_threads(dev, ops):
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_few_channels_with_steps_far_apart(dev, ops, dtype):
     """Steps of megabytes, so that a piece reaches beyond 32-bit offsets, in the workspace that was asked for."""
-    t, d, step = 2500, 8, 1_200_000
-    base = torch.zeros(t * step + d, device="cuda", dtype=DT[dtype])
+    t, d, step = (2500, 8, 1_200_000) if dtype == "f16" else (1000, 64, 2_100_000)
+    base = torch.zeros(t * step + 1000, device="cuda", dtype=DT[dtype])
     gate, x, gh = sequences(1, t, d, dtype, 3, True)
     far = [base[i * 64:].as_strided((1, t, d), (0, step, 1)) for i in range(6)]
     for a, b in zip(far, (gate, x, gh)):
