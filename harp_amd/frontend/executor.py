@@ -128,6 +128,9 @@ def _run_operators(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
         keep.append(memo)
         return out
 
+    def dense(g: GraphNode) -> GraphNode:
+        return g if g.view == View.contiguous(g.shape()) and g.op.kind != "view" else g.contiguous()
+
     def evaluate(nodes: Sequence[GraphNode]) -> None:
         """Dense buffers for `nodes`, whose graphs have no call left."""
         todo = []
@@ -141,34 +144,39 @@ def _run_operators(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
                     todo.append(n)
         if not todo:
             return
-        graphs = [g if g.view == View.contiguous(g.shape()) and g.op.kind != "view" else g.contiguous() for g in rebuilt(todo)]
-        for n, buf in zip(todo, _execute(graphs, buffers, fuse_program, constants, owned)):
+        for n, buf in zip(todo, _execute([dense(g) for g in rebuilt(todo)], buffers, fuse_program, constants, owned)):
             if buf is None:
                 raise ExecutionError("Internal: No output buffer returned from execution")
             put(n, buf)
 
     calls = []
+    depth: Dict[int, int] = {}                       # calls behind one another in a node's graph
     for n in topological_sort(roots):
+        depth[id(n)] = max([depth[id(s)] for s in n.src], default=0) + (1 if n.op.kind == "operator" else 0)
         if n.op.kind == "operator" and all(n.op.call is not c for c in calls):
             calls.append(n.op.call)
-    depth: Dict[int, int] = {}                       # calls behind one another in a node's graph
-
-    def depth_of(n: GraphNode) -> int:
-        for m in topological_sort([n]):
-            if id(m) not in depth:
-                depth[id(m)] = max([depth[id(s)] for s in m.src], default=0) + (1 if m.op.kind == "operator" else 0)
-        return depth[id(n)]
     stages: Dict[int, list] = {}
     for c in calls:
-        stages.setdefault(depth_of(c.nodes[0]), []).append(c)
+        stages.setdefault(max(depth[id(s)] for s in c.src) + 1, []).append(c)
     for d in sorted(stages):
         evaluate([s for c in stages[d] for s in c.src])
         for c in stages[d]:
             ins = [(buffers[id(values[key(s)])], [int(e.evaluate()) for e in s.shape()], s.dtype) for s in c.src]
             for node, buf in zip(c.nodes, dev.run_operator(c.name, c.attrs, ins, c.outputs)):
                 put(node, buf)
+
+    # A root that is a view is found by the name of the kernel's buffer that it views.  One of an input, or of what an
+    # earlier stage has computed, has none, and the lookup would fall back to another root's: it is copied, as
+    # every view of an operator's outputs is.  Other views stay what they are in a graph without operators.
+    def final(r: GraphNode, g: GraphNode) -> GraphNode:
+        below = r
+        while below.op.kind == "view" and below.src:
+            below = below.src[0]
+        if depth[id(r)] or (below is not r and below.is_external()):
+            return dense(g)
+        return g if below is r else r
     rest = [r for r in roots if r.op.kind != "operator"]
-    results = iter(_execute(rebuilt(rest), buffers, fuse_program, constants, owned) if rest else [])
+    results = iter(_execute([final(r, g) for r, g in zip(rest, rebuilt(rest))], buffers, fuse_program, constants, owned) if rest else [])
     return [buffers[id(values[key(r)])] if r.op.kind == "operator" else next(results) for r in roots]
 
 

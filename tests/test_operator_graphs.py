@@ -197,6 +197,72 @@ def test_a_recurrent_model_learns_from_a_teacher(fe):
         assert np.all(np.abs(entropy.to_numpy() + (np.exp(lp) * lp).sum(1)) < 1e-4)
 
 
+def many(fe, *tensors):
+    """Realized together; each as its shape says."""
+    fe.tensor.realize_many(tensors)
+    return [t.to_numpy().reshape(t.shape()) for t in tensors]
+
+
+def test_views_of_outputs_realized_with_other_roots(fe):
+    """A root that is a view of an operator's output, or of what one is computed into, has its own values, in the
+    view's order, whatever else is realized with it."""
+    rng = np.random.default_rng(7)
+    z, t = rng.normal(0, 2, (4, 9)).astype(np.float32), np.array([0, 3, 8, 5], np.int32)
+    logp, entropy = fe.nn.token_logprobs(tensor(fe, z), tensor(fe, t))
+    lp, as_square, total, e = many(fe, logp, logp.reshape([2, 2]), logp + entropy, entropy)
+    assert np.array_equal(as_square, lp.reshape(2, 2)) and np.array_equal(total, lp + e)
+    a = rng.uniform(0.1, 0.9, (2, 3, 4)).astype(np.float32)
+    g = tensor(fe, a)
+    h = fe.nn.gated_scan(g, g)
+    want = values(h)
+    twice = h + h
+    views = [h.permute([0, 2, 1]), twice.permute([2, 1, 0]), h.reshape([6, 4]), h.unsqueeze(0).expand(0, 2), -h.permute([1, 0, 2])]
+    wanted = [want.transpose(0, 2, 1), (want + want).transpose(2, 1, 0), want.reshape(6, 4), np.stack([want, want]), -want.transpose(1, 0, 2)]
+    for got, w in zip(many(fe, *views, h * h, h), wanted + [want * want, want]):
+        assert np.array_equal(got, w)
+    for v, w in zip(views, wanted):                                  # and alone
+        v.clear_buffer()
+        assert np.array_equal(values(v), w)
+
+
+def test_an_operators_source_and_its_views_as_roots(fe):
+    """What an operator reads is computed before it; as a root, and as a view in a root, it is still found, and so is
+    a view of an input.  What is computed of inputs alone is what it is without operators."""
+    rng = np.random.default_rng(8)
+    a, b = rng.uniform(0.1, 0.9, (2, 3, 4)).astype(np.float32), rng.uniform(0.1, 0.9, (2, 3, 4)).astype(np.float32)
+    ta, tb = tensor(fe, a), tensor(fe, b)
+    gate = ta * tb
+    h = fe.nn.gated_scan(gate, tb)
+    flat, swapped = gate.reshape([6, 4]), gate.permute([0, 2, 1])
+    swapped.realize()
+    before = swapped.to_numpy()
+    swapped.clear_buffer()
+    fe.tensor.realize_many([gate, flat, swapped, tb.reshape([4, 6]), h, h + gate])
+    x = a * b
+    assert np.array_equal(gate.to_numpy().reshape(x.shape), x) and np.array_equal(flat.to_numpy(), x.ravel())
+    assert np.array_equal(swapped.to_numpy(), before)
+    got = many(fe, tb.reshape([4, 6]), ta.permute([2, 0, 1]), h * h, h)
+    assert np.array_equal(got[0], b.reshape(4, 6)) and np.array_equal(got[1], a.transpose(2, 0, 1)) and np.array_equal(got[2], got[3] * got[3])
+
+
+@pytest.mark.parametrize("exact", [True, False])
+def test_gradients_behind_a_reshape_realized_together(fe, exact):
+    """The gradients of a step, which are views of one backward call's outputs, from one `realize_many`."""
+    rng = np.random.default_rng(9)
+    a, b, w = (rng.uniform(0.2, 0.9, (4, 2)).astype(np.float32) for _ in range(3))
+    params = [tensor(fe, x, True) for x in (a, b, w)]
+    with fe.exact_mode(exact):
+        h = fe.nn.gated_scan(params[0].reshape([1, 4, 2]), params[1].reshape([1, 4, 2])).reshape([4, 2])
+        loss = (h * params[2]).sum(1).sum(0)
+        loss.backward_with_params(params)
+        together = many(fe, *[p.grad() for p in params], loss)
+    states = oracle.scan(a[None], b[None], None, None, False)[0][0]
+    dg, dx, _ = oracle.scan_grad(a[None], states[None], w[None].astype(np.float64), None, None, False, None)[0]
+    # sums of four terms below 4, a dozen roundings each
+    for got, want in zip(together, (dg[0], dx[0], states, (states * w).sum())):
+        assert np.all(np.abs(got - want) <= 12 * 4 * 2.0 ** -24)
+
+
 @pytest.mark.parametrize("bad", [
     lambda fe, z, t, s: fe.nn.token_logprobs(z, t.cast(fe.F32)),
     lambda fe, z, t, s: fe.nn.token_logprobs(z, tensor(fe, np.zeros(3, np.int32))),
