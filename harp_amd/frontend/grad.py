@@ -97,7 +97,10 @@ def backward(output: GraphNode, params: Sequence[GraphNode], exact: bool = False
                 have = grads[node.op.index]
                 grads[node.op.index] = g if have is None else have + g
             waiting[id(call)] -= 1
-            if waiting[id(call)] == 0 and call.vjp is not None and any(x is not None for x in grads):
+            if waiting[id(call)] == 0 and any(x is not None for x in grads) and any(needs_grad(s) for s in call.src):
+                if call.vjp is None:
+                    raise NotImplementedError(f"'{call.name}' has no derivative: gradients through an operator are "
+                                              "taken once")
                 for src, gi in zip(call.src, call.vjp(grads)):
                     if gi is not None and needs_grad(src):
                         ctx.accumulate_grad(src, gi)

@@ -65,7 +65,7 @@ class OperatorCall:
     """One call of a backend's hand-written operator on dense tensors (not in the reference).  Its
     outputs are graph nodes of kind "operator" that share it; the executor runs the call between
     programs (see `executor.py`).  `vjp(grads)` takes a gradient per output (None where there is none)
-    and returns one per source."""
+    and returns one per source; without it differentiation through the call is refused."""
 
     __slots__ = ("name", "src", "attrs", "outputs", "vjp", "nodes")
 

@@ -207,7 +207,8 @@ def cross_entropy_loss(logits: Tensor, one_hot: Tensor, exact: bool = False) -> 
 # ---- language-model operators (harp_amd/operators.py) ---------------------------------------------------
 #
 # Nodes of the graph like any other, with gradients in both modes, but run between programs: a step
-# with one of them takes several programs, and `CompiledStep`, which is one, does not hold them.
+# with one of them takes several programs, and `CompiledStep`, which is one, does not hold them.  Their
+# gradients cannot be differentiated again; that is refused.
 
 
 def _f32(name: str, *tensors: Tensor) -> None:

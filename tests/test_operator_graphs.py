@@ -263,6 +263,31 @@ def test_gradients_behind_a_reshape_realized_together(fe, exact):
         assert np.all(np.abs(got - want) <= 12 * 4 * 2.0 ** -24)
 
 
+@pytest.mark.parametrize("exact", [True, False])
+def test_second_derivatives_are_refused(fe, exact):
+    """A gradient's own gradient through an operator is not there; the terms are not left out silently."""
+    rng = np.random.default_rng(10)
+    z, x = tensor(fe, rng.normal(0, 1, (3, 5)).astype(np.float32), True), tensor(fe, rng.uniform(0.2, 0.9, (1, 3, 2)).astype(np.float32), True)
+    w = tensor(fe, rng.normal(0, 1, (3, 5)).astype(np.float32), True)
+    one, other = tensor(fe, np.array([4, 0, 2], np.int32)), tensor(fe, np.array([[1, 2], [0, 3], [4, -1]], np.int32))
+    teacher = tensor(fe, rng.normal(0, 1, (3, 2)).astype(np.float32))
+
+    def total(t):
+        return t.reshape([int(np.prod(t.shape()))]).sum(0)
+    for p, y in ((z, fe.nn.token_logprobs(z, one)[0]), (z, fe.nn.token_logprobs(z, one)[1]), (z, fe.nn.distill_loss(z, teacher, other)),
+                 (x, fe.nn.gated_scan(x, x))):
+        with fe.exact_mode(exact):
+            p.zero_grad()
+            total(y * y).backward_with_params([p])
+            again = total(p.grad() * p.grad())
+            with pytest.raises(NotImplementedError, match="_backward' has no derivative"):
+                again.backward_with_params([p])
+            # by what the gradient does not depend on through the operator: ordinary
+            if p is z:
+                total(p.grad() * w).backward_with_params([w])
+                assert np.array_equal(values(w.grad()), values(p.grad().contiguous()))
+
+
 @pytest.mark.parametrize("bad", [
     lambda fe, z, t, s: fe.nn.token_logprobs(z, t.cast(fe.F32)),
     lambda fe, z, t, s: fe.nn.token_logprobs(z, tensor(fe, np.zeros(3, np.int32))),
