@@ -566,25 +566,26 @@ __device__ inline RowSums join_and_report(const DistillArgs& a, int64_t row, Row
   block_sum<THREADS>(r.s, kl, lds);
   if (threadIdx.x == 0) {
     const float log_s = log2_hw(r.s) * kLn2;
-    if (r.s == 0.f) kl = total != 0.f ? INFINITY : 0.f;
-    else kl += total * log_s;
-    a.loss[row] = kl * a.temperature * a.temperature;
+    if (r.s == 0.f) kl = INFINITY;
+    else kl += log_s;
+    // (a row without entries may hold anything, NaN among it)
+    a.loss[row] = total != 0.f ? kl * a.temperature * a.temperature : 0.f;
     a.norm[2 * row] = r.largest;
     a.norm[2 * row + 1] = log_s;
   }
   return r;
 }
 
-// dz_i = w T (Q p_i - sum_{k: id_k = i} q_k) with p_i = exp2(c2 (z_i - m) - log2 S).
+// dz_i = w T (p_i - sum_{k: id_k = i} q_k) with p_i = exp2(c2 (z_i - m) - log2 S), in rows that have entries.
 struct Gradient {
-  float w, coef, m, c2, shift;
-  __device__ Gradient(const DistillArgs& a, int64_t row, float m_, float log2_s, bool empty, float total)
-      : w(empty ? 0.f : (a.weight ? a.weight[row] : 1.f) * a.temperature), coef(empty ? 0.f : w * total), m(empty ? INFINITY : m_),
-        c2(a.in.scale * kLog2e), shift(empty ? 0.f : log2_s) {}
+  float w, m, c2, shift;
+  __device__ Gradient(const DistillArgs& a, int64_t row, float m_, float log2_s, bool empty)
+      : w(empty ? 0.f : (a.weight ? a.weight[row] : 1.f) * a.temperature), m(empty ? INFINITY : m_), c2(a.in.scale * kLog2e),
+        shift(empty ? 0.f : log2_s) {}
   // from the pair that the loss left
-  __device__ Gradient(const DistillArgs& a, int64_t row, float total)
-      : Gradient(a, row, a.norm[2 * row], a.norm[2 * row + 1] * kLog2e, a.norm[2 * row] == -INFINITY && a.norm[2 * row + 1] == -INFINITY, total) {}
-  __device__ float operator()(float z) const { return coef * exp2_hw(__builtin_fmaf(z - m, c2, -shift)); }
+  __device__ Gradient(const DistillArgs& a, int64_t row)
+      : Gradient(a, row, a.norm[2 * row], a.norm[2 * row + 1] * kLog2e, a.norm[2 * row] == -INFINITY && a.norm[2 * row + 1] == -INFINITY) {}
+  __device__ float operator()(float z) const { return w * exp2_hw(__builtin_fmaf(z - m, c2, -shift)); }
 };
 
 // The entries that the teacher names, by the threads that have written those elements without them: a
@@ -592,6 +593,14 @@ struct Gradient {
 template <int DT>
 __device__ inline void write_named(const Teacher& t, const Gradient& g, typename Elem<DT>::T* out) {
   for (int k = t.head[threadIdx.x]; k >= 0; k = t.next[k]) out[t.ids[k]] = Elem<DT>::put(g(t.z[k]) - g.w * t.sum[k]);
+}
+
+// The gradient of a row without entries, whatever its logits are.
+template <int DT, int THREADS> __device__ inline void clear_row(typename Elem<DT>::T* out, int n) {
+  constexpr int N = Elem<DT>::N;
+  const int full = n / N;
+  for (int i = threadIdx.x; i < full; i += THREADS) store16(out + static_cast<int64_t>(i) * N, u32x4{0, 0, 0, 0});
+  if (const int i = full * N + static_cast<int>(threadIdx.x); i < n) out[i] = Elem<DT>::put(0.f);
 }
 
 // A row to a workgroup, in its registers (THREADS * NV vectors) from one reading: the loss and the
@@ -656,7 +665,11 @@ template <int DT, int THREADS, int NV, int EX> __global__ __launch_bounds__(THRE
   const float z[4] = {last, -INFINITY, -INFINITY, -INFINITY};
   add_elements<4, false>(mine, z, c2);
   const RowSums r = join_and_report<DT, THREADS>(a, row, mine, zk, total, teacher, lds);
-  const Gradient gradient(a, row, r.m, log2_hw(r.s), r.s == 0.f, total);
+  if (total == 0.f) {
+    clear_row<DT, THREADS>(out, n);
+    return;
+  }
+  const Gradient gradient(a, row, r.m, log2_hw(r.s), r.s == 0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (i * THREADS >= full) break;
@@ -699,7 +712,7 @@ template <int DT> __global__ __launch_bounds__(256) void distill_stream(DistillA
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = j < n ? Elem<DT>::get(p[j]) : 0.f;
   }
-  const Gradient gradient(a, row, 1.f);
+  const Gradient gradient(a, row);
 #pragma unroll
   for (int j = 0; j < N; ++j) z[j] = gradient(z[j]);
   if (n >= N) {
@@ -717,15 +730,12 @@ template <int DT, int THREADS> __global__ __launch_bounds__(THREADS) void distil
   const Entry first(a, row, threadIdx.x);
   const float zk = student<DT>(a, row, first.id);
   const float total = load_teacher<THREADS, Elem<DT>::N, true>(a, row, first, teacher, lds);
-  const Gradient gradient(a, row, total);
   auto* out = static_cast<typename Elem<DT>::T*>(a.grad) + row * a.grad_stride;
   if (total == 0.f) {
-    constexpr int N = Elem<DT>::N;
-    const int full = a.in.vocab / N;
-    for (int i = threadIdx.x; i < full; i += THREADS) store16(out + static_cast<int64_t>(i) * N, u32x4{0, 0, 0, 0});
-    if (const int i = full * N + static_cast<int>(threadIdx.x); i < a.in.vocab) out[i] = Elem<DT>::put(0.f);
+    clear_row<DT, THREADS>(out, a.in.vocab);
     return;
   }
+  const Gradient gradient(a, row);
   for (int k = threadIdx.x; k < a.k; k += THREADS)
     if (const int id = teacher.ids[k]; id >= 0)
       out[id] = Elem<DT>::put(gradient(k < THREADS ? zk : student<DT>(a, row, id)) - gradient.w * teacher.sum[k]);

@@ -327,7 +327,7 @@ int eh_token_logprobs_backward(eh_device* dev, const eh_token_logprobs_backward_
  * teacher names in that row (k <= 1024).
  *   teacher    [rows][k]      f32, bf16 or f16 logits, any order; ids [rows][k] i32 or i64.  An id outside
  *                             [0, vocab) is no entry; a token named twice counts twice.  A row without
- *                             entries has loss 0 and gradient 0
+ *                             entries has loss 0 and gradient 0, whatever its logits are (NaN, say)
  *   loss       [rows] f32, norm [rows][2] f32 (as above, with scale 1 / T)
  *   grad       [rows][vocab] of the logits' type, or absent: weight_r times the gradient of loss_r,
  *                             weight_r T (p_i - sum of q over the entries that name i)

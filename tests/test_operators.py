@@ -305,6 +305,38 @@ def test_distill_edges(dev, ops, v, dtype):
     assert loss[5] == np.inf and not grad[5].any() and loss[6] == 0 and not grad[6].any() and loss[7] == np.inf
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,v", [(6, 40), (6, 5003), (6, 60000), (6, 400007), (300, 200003)])
+def test_distill_rows_without_entries_may_hold_anything(dev, ops, n, v, dtype):
+    """Loss 0 and gradient 0, held in registers, in segments, and read twice: NaN, infinities, all of one kind."""
+    z = rows_of(n, v, dtype, 5)
+    ids = torch.full((n, 3), -1, device="cuda")
+    ids[:, 1:] = torch.tensor([v, -7], device="cuda")
+    ids[2] = torch.tensor([0, 1, 2], device="cuda")            # (no entry either: the teacher's logits are -infinity)
+    ids[5] = torch.tensor([v - 1, 3, 3], device="cuda")        # the one row with entries
+    u = on_gpu(np.random.default_rng(0).normal(0, 1, (n, 3)).astype(np.float32))
+    u[2] = -np.inf
+    z[0, v // 2] = np.nan
+    z[1] = np.nan
+    z[2, 1] = np.inf
+    z[3] = np.inf
+    z[4] = -np.inf
+    weight = on_gpu(np.linspace(-1, 2, n).astype(np.float32))
+    full = lambda *s, dt=torch.float32: torch.full(s, 7.0, device="cuda", dtype=dt)  # noqa: E731
+    out = ops.Distilled(full(n), full(n, 2), full(n, v, dt=DT[dtype]))
+    ops.distill_loss(dev, z, u, ids, temperature=1.5, row_weight=weight, grad=True, out=out)
+    alone = ops.Distilled(full(n), full(n, 2), None)
+    ops.distill_loss(dev, z, u, ids, temperature=1.5, out=alone)
+    later = ops.distill_loss_backward(dev, z, u, ids, out.norm, weight, temperature=1.5, out=full(n, v, dt=DT[dtype]))
+    none = [i for i in range(n) if i != 5]
+    for loss in (out.loss, alone.loss):
+        assert not host(loss)[none].any() and np.isfinite(host(loss)[5]) and host(loss)[5] != 0
+    for grad, norm in ((out.grad, None), (later, host(out.norm[5:6]))):
+        assert not bool(grad[none].any())
+        want, tol = oracle.distill(host(z[5:6]), host(u[5:6]), ids[5:6].cpu().numpy(), 1.5, host(weight[5:6]), norm=norm)[4:]
+        close(host(grad[5:6]), want, tol + oracle.rounding(dtype, want), "grad")
+
+
 def test_distill_gradient_against_differences(dev, ops):
     """As for the scores; the third derivative of T^2 KL by a logit is below 1 / T."""
     rng = np.random.default_rng(2)
