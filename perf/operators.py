@@ -15,7 +15,7 @@ own = False
 _DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 _SIZE = {"f32": 4, "bf16": 2, "f16": 2}
 IGNORE = -1
-_handle = None
+_handles = {}
 
 
 def listed():
@@ -188,17 +188,22 @@ def run(state):
     return {"score": _score, "score_grad": _score_grad, "distill": _distill, "distill_grad": _distill_grad, "scan": _scan, "scan_grad": _scan_grad}[state["case"]["op"]](state)
 
 
-def _device():
-    global _handle
-    if _handle is None:
+def _device(x):
+    """The device handle of the stream that torch works on now, on the GPU of `x`.  (The stream as a number: as an object of
+    torch's it takes 2.7 us, a third of the smallest calls.)"""
+    index = x.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    handle = _handles.get((index, stream))
+    if handle is None:
         from harp_amd.backend import HipDevice
-        _handle = HipDevice(torch.cuda.current_device(), stream=torch.cuda.current_stream().cuda_stream)
-    return _handle
+        handle = _handles[index, stream] = HipDevice(index, stream=stream)
+    return handle
 
 
 def _own(st):
     from harp_amd import operators as ops
-    dev, case = _device(), st["case"]
+    case = st["case"]
+    dev = _device(st["gate"] if "gate" in st else st["logits"])
     op = case["op"]
     if op == "score":
         out = ops.Logprobs(st["logp"], st["entropy"], st["norm"], st["top_logp"], st["top_ids"])
