@@ -185,6 +185,28 @@ Binary HipCompiler::compile(const std::string& source, const std::string& arch, 
 // HipDevice / HipBuffer / HipKernel
 // ---------------------------------------------------------------------------------------------
 
+// A word of pinned host memory for a handle of the current device, `index`.  A device's words are never freed:
+// kernels of a graph that outlives its handle still have the address.  The 1025th handle shares the first one's.
+static unsigned int* wait_word(int index) {
+  constexpr size_t kWords = 1024, kStride = 16;
+  static std::mutex mu;
+  static std::map<int, std::pair<unsigned int*, size_t>> blocks;
+  std::lock_guard<std::mutex> lk(mu);
+  auto& b = blocks[index];
+  if (!b.first) {
+    // (a handle may be opened while some thread captures a graph)
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    check(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode");
+    void* p = nullptr;
+    const hipError_t e = hipHostMalloc(&p, kWords * kStride * sizeof(unsigned int), hipHostMallocDefault);
+    check(hipThreadExchangeStreamCaptureMode(&mode), "hipThreadExchangeStreamCaptureMode");
+    check(e, "hipHostMalloc");
+    std::memset(p, 0, kWords * kStride * sizeof(unsigned int));
+    b.first = static_cast<unsigned int*>(p);
+  }
+  return b.first + (b.second++ % kWords) * kStride;
+}
+
 int HipDevice::count() {
   int n = 0;
   if (hipGetDeviceCount(&n) != hipSuccess) {
@@ -228,6 +250,8 @@ void HipDevice::open() {
   profile_.memory_bus_bits = p.memoryBusWidth;
   profile_.l2_bytes = p.l2CacheSize;
   pool_limit_ = std::getenv("ECLAT_HIP_NO_POOL") ? 0 : profile_.global_memory_size / 4;
+  lost_wait_ = wait_word(index_);
+  if (const char* polls = std::getenv("ECLAT_HIP_WAIT_POLLS")) wait_polls_ = std::clamp(std::atoi(polls), 0, 1 << 22);
   // resolved here, with this device current, so that the entry point which must not allocate
   // never triggers the load of the library's code object itself
   try {
@@ -380,6 +404,7 @@ void HipBuffer::read_to_host(void* dst, size_t bytes) const {
   dev_->make_current();
   check(hipMemcpyAsync(dst, ptr_, bytes_, hipMemcpyDeviceToHost, dev_->stream()), "hipMemcpyAsync(D2H)");
   check(hipStreamSynchronize(dev_->stream()), "hipStreamSynchronize");
+  dev_->check_waits();
 }
 
 void HipBuffer::copy_from(const HipBuffer& src) {

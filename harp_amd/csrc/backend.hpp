@@ -71,6 +71,16 @@ class HipDevice {
   const DeviceProfile& profile() const { return profile_; }
   void make_current() const;
   void synchronize() const;
+  // A kernel whose workgroups wait for each other gives up after `wait_polls` looks and leaves a 1 in
+  // `lost_wait`, a word of pinned host memory that outlives the handle (a graph may be replayed after it).
+  // `check_waits` reports that once, as an error.
+  unsigned int* lost_wait() const { return lost_wait_; }
+  int wait_polls() const { return wait_polls_; }
+  void check_waits() const {
+    if (lost_wait_ && __atomic_exchange_n(lost_wait_, 0u, __ATOMIC_ACQ_REL))
+      throw Error("gated_scan: a workgroup has waited in vain for another one's part of its sequence (hip error), as when two "
+                  "calls work in one workspace at once; what that call wrote is not to be used");
+  }
 
   // Loads a code object and resolves one entry point; modules are shared per (binary, entry).
   std::shared_ptr<HipKernel> load(const Binary& bin, const std::string& entry);
@@ -102,6 +112,8 @@ class HipDevice {
   size_t pooled_bytes_ = 0, pool_limit_ = 0;
   void* static_scratch_ = nullptr;
   std::string static_scratch_error_;
+  unsigned int* lost_wait_ = nullptr;
+  int wait_polls_ = 1 << 22;           // seconds
 };
 
 class HipBuffer {

@@ -154,7 +154,10 @@ int eh_device_get_props(eh_device* dev, eh_device_props* out) {
 
 int eh_device_sync(eh_device* dev) {
   REQUIRE(dev, "device is NULL");
-  return guard([&] { dev->dev.synchronize(); });
+  return guard([&] {
+    dev->dev.synchronize();
+    dev->dev.check_waits();
+  });
 }
 
 int eh_device_stream(eh_device* dev, void** stream) {

@@ -37,12 +37,15 @@ __device__ inline unsigned int word_of(float x) {
 
 // A word of the board once it is there.  That every wait ends follows from the order of the tickets; one that
 // has lasted for seconds all the same (two calls in one workspace at once, say) ends with the
-// empty word, which is NaN.
-template <class Word> __device__ inline Word wait_for(const Word* p) {
-  Word w;
-  for (int i = 0; (w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == static_cast<Word>(~0ull) && i < 1 << 22; ++i)
+// empty word, which is NaN, and tells the host.
+template <class Word> __device__ inline Word wait_for(const ScanArgs& a, const Word* p) {
+  for (int i = 0; i < a.polls; ++i) {
+    const Word w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (w != static_cast<Word>(~0ull)) return w;
     __builtin_amdgcn_s_sleep(1);
-  return w;
+  }
+  __hip_atomic_store(a.lost, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  return static_cast<Word>(~0ull);
 }
 
 // A row of at least a vector is read by the vector that ends with it, which `down` channels are moved out of: by
@@ -305,7 +308,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     for (int i = 0; i < M; ++i) {
       const int q = p + i * (P / M);
       if (!mine || q >= member) break;
-      const unsigned long long w = wait_for(words - static_cast<int64_t>(member - q) * CW);
+      const unsigned long long w = wait_for(a, words - static_cast<int64_t>(member - q) * CW);
       others[0][q][c] = __uint_as_float(static_cast<unsigned int>(w >> 32));
       others[1][q][c] = __uint_as_float(static_cast<unsigned int>(w));
     }
@@ -315,7 +318,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     if (behind < P) {
       h = start ? start[b * a.width + tile + c] : 0.f;
     } else {
-      h = __uint_as_float(wait_for(board.states + (group - 1) * CW + c));
+      h = __uint_as_float(wait_for(a, board.states + (group - 1) * CW + c));
     }
     before[c] = h;
   }

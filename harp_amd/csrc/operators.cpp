@@ -426,6 +426,8 @@ static ScanArgs scan_sizes(const HipDevice& d, int64_t batch, int64_t time, int6
   if (!is_float(gate.dtype)) throw Error("gate: has to be f32, bf16 or f16");
   ScanArgs s{};
   s.compute_units = units(d);
+  s.polls = d.wait_polls();
+  s.lost = d.lost_wait();
   s.batch = batch, s.time = time, s.width = static_cast<int>(width);
   s.dtype = static_cast<int>(gate.dtype);
   s.log_gate = log_gate != 0;
@@ -454,6 +456,7 @@ int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync) {
   return guard([&] {
     const eh_gated_scan_args& a = *args;
     HipDevice* d = &dev->dev;
+    d->check_waits();
     ScanArgs s = scan_sizes(*d, a.batch, a.time, a.width, a.log_gate, a.gate);
     auto lk = d->stream_lock();
     Current current(d);
@@ -471,7 +474,9 @@ int eh_gated_scan(eh_device* dev, const eh_gated_scan_args* args, int sync) {
     arrays.settle();
     if (a.batch) launched(launch_scan(s, d->stream()), "launch of gated_scan");
     arrays.written();
-    if (sync) d->synchronize();
+    if (!sync) return;
+    d->synchronize();
+    d->check_waits();
   });
 }
 
@@ -480,6 +485,7 @@ int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* ar
   return guard([&] {
     const eh_gated_scan_backward_args& a = *args;
     HipDevice* d = &dev->dev;
+    d->check_waits();
     ScanArgs s = scan_sizes(*d, a.batch, a.time, a.width, a.log_gate, a.gate);
     auto lk = d->stream_lock();
     Current current(d);
@@ -500,7 +506,9 @@ int eh_gated_scan_backward(eh_device* dev, const eh_gated_scan_backward_args* ar
     arrays.settle();
     if (a.batch) launched(launch_scan_grad(s, d->stream()), "launch of gated_scan_backward");
     arrays.written();
-    if (sync) d->synchronize();
+    if (!sync) return;
+    d->synchronize();
+    d->check_waits();
   });
 }
 

@@ -760,6 +760,48 @@ def test_few_channels_with_steps_far_apart(dev, ops, dtype):
         close(host(got), w, tl + oracle.rounding(dtype, w), name)
 
 
+def test_a_wait_given_up_is_reported(dev, ops, monkeypatch):
+    """A scan whose workgroups do not look for each other's parts at all (a limit of no looks, set from the host): the call
+    ends, what follows the first piece is NaN, and the handle says so once, wherever it next waits or scans."""
+    from harp_amd import backend as hb
+    from harp_amd.frontend import F32
+    gate, x, grad_h = sequences(1, 2000, 64, "f32", 5, True)
+    h, fin = torch.empty_like(x), torch.empty(1, 64, device="cuda")
+    grads = ops.ScanGrads(torch.empty_like(x), torch.empty_like(x), None)
+    monkeypatch.setenv("ECLAT_HIP_WAIT_POLLS", "0")
+    mine = hb.HipDevice(0, stream=torch.cuda.current_stream().cuda_stream)
+    monkeypatch.delenv("ECLAT_HIP_WAIT_POLLS")
+    some = hb.HipBuffer(mine, [4], F32)
+    some.write_array(np.zeros(4, np.float32))
+
+    def scan():
+        ops.gated_scan(mine, gate, x, log_gate=True, out=h, final=fin)
+
+    def back():
+        ops.gated_scan_backward(mine, gate, h, grad_h, log_gate=True, out=grads)
+    for call, follows in ((scan, mine.sync), (back, mine.sync), (scan, lambda: some.read_array(np.float32))):
+        call()
+        with pytest.raises(hb.EhError, match="in vain"):
+            follows()
+        follows()
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(h[:, :512]).all()) and bool(torch.isnan(h[:, 512:]).all()) and bool(torch.isnan(fin).all())
+    for follows in (scan, back):                                   # the next scan is not queued
+        scan()
+        torch.cuda.synchronize()
+        h.zero_()
+        with pytest.raises(hb.EhError, match="in vain"):
+            follows()
+        torch.cuda.synchronize()
+        assert not bool(h.any())
+    dev.sync()                                                       # another handle has lost nothing
+    ops.gated_scan(dev, gate, x, log_gate=True, out=h, final=fin)
+    want, tol, _, _ = oracle.scan(host(gate), host(x), None, None, True)
+    close(host(h), want, tol, "h")
+    dev.sync()
+    mine.sync()
+
+
 REFUSED = [
     ("overlap", lambda o, d, z, t, e: o.token_logprobs_backward(d, z, t, e(4, 2), out=z)),
     ("overlap", lambda o, d, z, t, e: o.gated_scan(d, z[None], z[None], out=z[None])),
