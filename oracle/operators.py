@@ -1,4 +1,4 @@
-"""The front end's operators on the CPU oracle: their definitions in 64 bits, rounded to f32 at the end.
+"""The front end's operators on the CPU oracle: their definitions (include/eclat_hip.h) in 64 bits, rounded to f32 at the end.
 Test infrastructure, like the rest of this package."""
 
 from __future__ import annotations
@@ -14,9 +14,17 @@ def _array(item):
 
 
 def _log_softmax(z, scale):
+    """Largest logit, log of the sum, log probabilities (-inf throughout a row without a logit above -infinity)."""
     m = z.max(1, keepdims=True)
-    d = scale * (z - m)
-    return m, np.log(np.exp(d).sum(1, keepdims=True)), d
+    empty = m == -np.inf
+    d = scale * (z - np.where(empty, 0.0, m))
+    log_s = np.log(np.exp(d).sum(1, keepdims=True))
+    return m, log_s, np.where(empty, -np.inf, d - log_s)
+
+
+def _times_log(p, x):
+    """p x, 0 where p is 0."""
+    return np.where(p == 0, 0.0, p * x)
 
 
 def _teacher(u, ids, v, temperature):
@@ -29,38 +37,49 @@ def _teacher(u, ids, v, temperature):
 
 
 def compute(name, attrs, arrays):
+    with np.errstate(all="ignore"):
+        return _compute(name, attrs, arrays)
+
+
+def _compute(name, attrs, arrays):
     f = [a.astype(np.float64) if a.dtype.kind == "f" else a for a in arrays]
     if name.startswith("token_logprobs"):
         z, t = f[0], f[1]
-        c, n = attrs["scale"], z.shape[0]
+        c, (n, v) = attrs["scale"], z.shape
         live = t != attrs["ignore_index"]
-        at = np.where(live, t, 0)
+        inside = (t >= 0) & (t < v)
+        at = np.where(inside, t, 0)
         if name == "token_logprobs":
-            m, log_s, d = _log_softmax(z, c)
-            lp = d - log_s
-            return [np.where(live, lp[np.arange(n), at], 0.0), -(np.exp(lp) * lp).sum(1), np.concatenate([m, log_s], 1)]
+            m, log_s, lp = _log_softmax(z, c)
+            p = np.exp(lp)
+            return [np.where(live, np.where(inside, lp[np.arange(n), at], np.nan), 0.0), -_times_log(p, lp).sum(1), np.concatenate([m, log_s], 1)]
         norm, entropy, grads = f[2], f[3], list(f[4:])
         g = np.where(live, grads.pop(0), 0.0) if attrs["logp"] else np.zeros(n)
+        g = np.where(live & ~inside, np.nan, g)
         e = grads.pop(0) if attrs["entropy"] else np.zeros(n)
+        empty = (norm == -np.inf).all(1)
         lp = c * (z - norm[:, :1]) - norm[:, 1:]
         p = np.exp(lp)
         hot = np.zeros_like(z)
-        hot[np.arange(n), at] = 1.0
-        return [c * (g[:, None] * (hot - p) - e[:, None] * p * (lp + entropy[:, None]))]
+        hot[np.arange(n), at] = live & inside
+        grad = c * (g[:, None] * (hot - p) - e[:, None] * _times_log(p, lp + entropy[:, None]))
+        return [np.where(empty[:, None], 0.0, grad)]
     if name.startswith("distill_loss"):
         z, u, ids = f[0], f[1], f[2]
         n, v = z.shape
         temp = attrs["temperature"]
         q = _teacher(u, ids, v, temp)
+        none = (q == 0).all(1)
         at = np.clip(ids, 0, v - 1)
         if name == "distill_loss":
-            m, log_s, d = _log_softmax(z, 1.0 / temp)
-            lp = np.take_along_axis(d - log_s, at, 1)
-            return [temp * temp * (np.where(q > 0, q * (np.log(np.where(q > 0, q, 1.0)) - lp), 0.0)).sum(1), np.concatenate([m, log_s], 1)]
+            m, log_s, lp = _log_softmax(z, 1.0 / temp)
+            lp = np.take_along_axis(lp, at, 1)
+            loss = temp * temp * _times_log(q, np.log(q) - lp).sum(1)
+            return [np.where(none, 0.0, loss), np.concatenate([m, log_s], 1)]
         norm, g = f[3], f[4]
-        grad = np.exp((z - norm[:, :1]) / temp - norm[:, 1:]) * q.sum(1, keepdims=True)
+        grad = np.exp((z - norm[:, :1]) / temp - norm[:, 1:])
         np.add.at(grad, (np.arange(n)[:, None], at), -q)
-        return [g[:, None] * temp * grad]
+        return [np.where((none | (norm == -np.inf).all(1))[:, None], 0.0, g[:, None] * temp * grad)]
     gate = np.exp(f[0]) if attrs["log_gate"] else f[0]
     b, t, d = gate.shape
     if name == "gated_scan":

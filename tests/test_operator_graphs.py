@@ -288,6 +288,47 @@ def test_second_derivatives_are_refused(fe, exact):
                 assert np.array_equal(values(w.grad()), values(p.grad().contiguous()))
 
 
+def same(got, want, tol):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    with np.errstate(invalid="ignore"):
+        return np.all((np.isnan(got) & np.isnan(want)) | (got == want) | (np.abs(got - want) <= tol + 2.0 ** -24 * np.abs(want)))
+
+
+def test_masked_rows_and_ids_outside_the_vocabulary(fe):
+    """Tokens that cannot occur, rows of nothing else, targets that are no token, rows without the teacher's entries."""
+    rng = np.random.default_rng(11)
+    z = rng.normal(0, 2, (6, 13)).astype(np.float32)
+    z[0, ::2] = -np.inf
+    z[1] = -np.inf
+    z[2, 1:] = -np.inf
+    t = np.array([1, 4, 0, 13, -7, -1], np.int64)
+    logits = tensor(fe, z, True)
+    logp, entropy = fe.nn.token_logprobs(logits, tensor(fe, t))
+    want = oracle.score(z, t, -1, 1.0, 0)
+    assert same(values(logp), want["logp"], want["logp_tol"]) and same(values(entropy), want["entropy"], want["entropy_tol"])
+    g, e = rng.normal(0, 1, 6).astype(np.float32), rng.normal(0, 1, 6).astype(np.float32)
+    with fe.exact_mode():
+        got = gradients(fe, (logp * tensor(fe, g) + entropy * tensor(fe, e)).sum(0), [logits])[0]
+    # the norm and the entropy that it reads are within their own bounds of these, and p |log p + H| is below 20
+    norm, ent = want["norm"].astype(np.float32), want["entropy"].astype(np.float32)
+    grad, tol = oracle.score_grad(z, t, -1, 1.0, norm, ent, g, e)
+    off = (np.abs(g) + 20 * np.abs(e))[:, None] * (want["norm_tol"][:, 1:] + want["entropy_tol"][:, None] + 2 * 2.0 ** -24 * 20)
+    assert same(got, grad, tol + off)
+
+    u, ids = rng.normal(0, 2, (6, 3)).astype(np.float32), np.array([[1, 3, 5], [0, 1, 2], [0, -1, 13], [2, 2, 3], [-1, 13, -9], [4, 5, -1]], np.int32)
+    z[4, 3] = np.nan
+    z[5, 4] = -np.inf
+    u[5, 0] = -np.inf
+    logits = tensor(fe, z, True)
+    loss = fe.nn.distill_loss(logits, tensor(fe, u), tensor(fe, ids))
+    want, loss_tol, _, norm_tol, grad, tol = oracle.distill(np.where(np.isnan(z), 0, z), u, ids, 1.0, None)
+    assert want[4] == 0 and want[1] == np.inf and np.isfinite(want[[0, 2, 3, 5]]).all() and not grad[[1, 4]].any()
+    assert same(values(loss), want, loss_tol)
+    with fe.exact_mode():
+        got = gradients(fe, loss.sum(0), [logits])[0]
+    assert same(got, grad, tol + norm_tol[:, 1:] + 2.0 ** -24 * 20)        # p is at most 1, its argument off by the norm's rounding
+
+
 @pytest.mark.parametrize("bad", [
     lambda fe, z, t, s: fe.nn.token_logprobs(z, t.cast(fe.F32)),
     lambda fe, z, t, s: fe.nn.token_logprobs(z, tensor(fe, np.zeros(3, np.int32))),
