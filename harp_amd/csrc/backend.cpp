@@ -251,7 +251,7 @@ void HipDevice::open() {
   profile_.l2_bytes = p.l2CacheSize;
   pool_limit_ = std::getenv("ECLAT_HIP_NO_POOL") ? 0 : profile_.global_memory_size / 4;
   lost_wait_ = wait_word(index_);
-  if (const char* polls = std::getenv("ECLAT_HIP_WAIT_POLLS")) wait_polls_ = std::clamp(std::atoi(polls), 0, 1 << 22);
+  lose_waits_ = std::getenv("ECLAT_HIP_LOSE_WAITS") != nullptr;
   // resolved here, with this device current, so that the entry point which must not allocate
   // never triggers the load of the library's code object itself
   try {

@@ -71,11 +71,11 @@ class HipDevice {
   const DeviceProfile& profile() const { return profile_; }
   void make_current() const;
   void synchronize() const;
-  // A kernel whose workgroups wait for each other gives up after `wait_polls` looks and leaves a 1 in
-  // `lost_wait`, a word of pinned host memory that outlives the handle (a graph may be replayed after it).
-  // `check_waits` reports that once, as an error.
+  // A kernel whose workgroups wait for each other leaves a 1 in `lost_wait`, a word of pinned host memory that
+  // outlives the handle (a graph may be replayed after it), when one of them has waited in vain.
+  // `check_waits` reports that once, as an error; `lose_waits` has a test see it.
   unsigned int* lost_wait() const { return lost_wait_; }
-  int wait_polls() const { return wait_polls_; }
+  bool lose_waits() const { return lose_waits_; }
   void check_waits() const {
     if (lost_wait_ && __atomic_exchange_n(lost_wait_, 0u, __ATOMIC_ACQ_REL))
       throw Error("gated_scan: a workgroup has waited in vain for another one's part of its sequence (hip error), as when two "
@@ -113,7 +113,7 @@ class HipDevice {
   void* static_scratch_ = nullptr;
   std::string static_scratch_error_;
   unsigned int* lost_wait_ = nullptr;
-  int wait_polls_ = 1 << 22;           // seconds
+  bool lose_waits_ = false;
 };
 
 class HipBuffer {

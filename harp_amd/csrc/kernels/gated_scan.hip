@@ -36,16 +36,14 @@ __device__ inline unsigned int word_of(float x) {
 }
 
 // A word of the board once it is there.  That every wait ends follows from the order of the tickets; one that
-// has lasted for seconds all the same (two calls in one workspace at once, say) ends with the
-// empty word, which is NaN, and tells the host.
-template <class Word> __device__ inline Word wait_for(const ScanArgs& a, const Word* p) {
-  for (int i = 0; i < a.polls; ++i) {
-    const Word w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (w != static_cast<Word>(~0ull)) return w;
+// has lasted for half a second all the same (two calls in one workspace at once, say) ends with the
+// empty word, which is NaN.
+template <class Word> __device__ inline Word wait_for(const Word* p) {
+  Word w;
+#pragma unroll 1
+  for (int left = 1 << 22; (w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == static_cast<Word>(~0ull) && --left;)
     __builtin_amdgcn_s_sleep(1);
-  }
-  __hip_atomic_store(a.lost, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  return static_cast<Word>(~0ull);
+  return w;
 }
 
 // A row of at least a vector is read by the vector that ends with it, which `down` channels are moved out of: by
@@ -308,7 +306,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     for (int i = 0; i < M; ++i) {
       const int q = p + i * (P / M);
       if (!mine || q >= member) break;
-      const unsigned long long w = wait_for(a, words - static_cast<int64_t>(member - q) * CW);
+      const unsigned long long w = wait_for(words - static_cast<int64_t>(member - q) * CW);
       others[0][q][c] = __uint_as_float(static_cast<unsigned int>(w >> 32));
       others[1][q][c] = __uint_as_float(static_cast<unsigned int>(w));
     }
@@ -318,7 +316,7 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
     if (behind < P) {
       h = start ? start[b * a.width + tile + c] : 0.f;
     } else {
-      h = __uint_as_float(wait_for(a, board.states + (group - 1) * CW + c));
+      h = __uint_as_float(wait_for(board.states + (group - 1) * CW + c));
     }
     before[c] = h;
   }
@@ -332,6 +330,14 @@ __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces
       if (a.final_state) a.final_state[b * a.width + tile + c] = next;
     } else if (member == P - 1) {
       __hip_atomic_store(board.states + group * CW + c, word_of(next), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    // NaN of its own, or a wait that gave up: the host is told.  (The state is looked up again; to keep its word from
+    // the first look would delay every piece, 1 x 131072 x 64 bf16 by 0.6 us of 29.)
+    if (W == 8 && pieces > 1 && next != next) {
+      bool lost = behind >= P && __hip_atomic_load(board.states + (group - 1) * CW + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == kEmpty;
+#pragma unroll 1
+      for (int i = 0; i < member; ++i) lost |= __float_as_uint(others[0][i][c]) == kEmpty;
+      if (lost) __hip_atomic_store(a.lost, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
   }
   __syncthreads();
@@ -471,6 +477,11 @@ template <int DT, int STEPS, bool BACK, bool LOG> __global__ __launch_bounds__(2
   for (int j = 0; j < N; j += 4) store16(a.final_state + end + j, Elem<kF32>::pack(h + j));
 }
 
+// For tests of what a lost wait leads to: every column's first turn is taken, by nobody.
+__global__ __launch_bounds__(64) void skip_turns(unsigned int* tickets, int64_t columns, int classes) {
+  if (static_cast<int>(threadIdx.x) < classes) tickets[threadIdx.x * kTicketStride] = static_cast<unsigned int>(Class(columns, classes, threadIdx.x).columns) - 1u;
+}
+
 __global__ __launch_bounds__(256) void clear_board(unsigned int* p, size_t n) {
   for (size_t i = blockIdx.x * size_t{256} + threadIdx.x; i < n; i += size_t{256} * gridDim.x) p[i] = kEmpty;
 }
@@ -507,6 +518,8 @@ template <bool BACK> hipError_t launch(const ScanArgs& a, hipStream_t stream) {
     board.states = reinterpret_cast<unsigned int*>(board.maps + a.batch * p.tiles * p.pieces * p.channels);
     const size_t blocks = (words + 1023) / 1024;
     if (hipError_t e = queue(clear_board, static_cast<unsigned>(blocks < 1024 ? blocks : 1024), 256, 0, stream, board.tickets, words)) return e;
+    if (a.lose_waits)
+      if (hipError_t e = queue(skip_turns, 1, 64, 0, stream, board.tickets, a.batch * p.tiles, p.classes)) return e;
   }
   const unsigned grid = static_cast<unsigned>(a.batch * p.tiles * p.pieces);
   return by_type(a.dtype, [&](auto dt) {

@@ -426,7 +426,7 @@ static ScanArgs scan_sizes(const HipDevice& d, int64_t batch, int64_t time, int6
   if (!is_float(gate.dtype)) throw Error("gate: has to be f32, bf16 or f16");
   ScanArgs s{};
   s.compute_units = units(d);
-  s.polls = d.wait_polls();
+  s.lose_waits = d.lose_waits();
   s.lost = d.lost_wait();
   s.batch = batch, s.time = time, s.width = static_cast<int>(width);
   s.dtype = static_cast<int>(gate.dtype);

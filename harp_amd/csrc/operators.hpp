@@ -126,8 +126,8 @@ struct ScanArgs {
   const int* lengths;          // [batch] or null
   int compute_units;
   void* workspace;
-  int polls;                   // after which a wait for another workgroup gives up,
-  unsigned int* lost;          // leaving a 1 here (host memory)
+  unsigned int* lost;          // receives a 1 from a workgroup that has waited for another one in vain (host memory)
+  bool lose_waits;             // (tests) leave a piece out, so that others wait for it in vain
 };
 // A workgroup of `waves` waves has `lanes` vectors of channels and a piece of waves * 64 / lanes * kScanSteps steps.
 constexpr int kScanSteps = 8;        // of a thread

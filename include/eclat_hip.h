@@ -353,7 +353,7 @@ int eh_distill_loss_backward(eh_device* dev, const eh_distill_loss_args* args, i
  *                    behind them is neither read nor written in any array
  * Products of gates are formed along a sequence, so gates are meant to be at most about 1 in magnitude: a
  * product that leaves f32's range gives what inf and 0 give.
- * Long sequences are the work of several workgroups, which wait for each other.  A wait that is in vain for seconds
+ * Long sequences are the work of several workgroups, which wait for each other.  A wait that is in vain for half a second
  * (two calls in one workspace at once, say) ends: the call's results hold NaN then and are not to be used, and
  * whichever comes first of the handle's next scan, eh_device_sync, eh_buffer_read or call with sync != 0 of a scan
  * returns EH_ERR_DEVICE, once. */

@@ -761,16 +761,15 @@ def test_few_channels_with_steps_far_apart(dev, ops, dtype):
 
 
 def test_a_wait_given_up_is_reported(dev, ops, monkeypatch):
-    """A scan whose workgroups do not look for each other's parts at all (a limit of no looks, set from the host): the call
-    ends, what follows the first piece is NaN, and the handle says so once, wherever it next waits or scans."""
+    """A scan whose first piece is left out (by the host), so that the others wait for it in vain: the call ends, what
+    follows is NaN, and the handle says so once, wherever it next waits or scans."""
     from harp_amd import backend as hb
     from harp_amd.frontend import F32
     gate, x, grad_h = sequences(1, 2000, 64, "f32", 5, True)
-    h, fin = torch.empty_like(x), torch.empty(1, 64, device="cuda")
-    grads = ops.ScanGrads(torch.empty_like(x), torch.empty_like(x), None)
-    monkeypatch.setenv("ECLAT_HIP_WAIT_POLLS", "0")
+    h, fin = torch.zeros_like(x), torch.zeros(1, 64, device="cuda")
+    monkeypatch.setenv("ECLAT_HIP_LOSE_WAITS", "1")
     mine = hb.HipDevice(0, stream=torch.cuda.current_stream().cuda_stream)
-    monkeypatch.delenv("ECLAT_HIP_WAIT_POLLS")
+    monkeypatch.delenv("ECLAT_HIP_LOSE_WAITS")
     some = hb.HipBuffer(mine, [4], F32)
     some.write_array(np.zeros(4, np.float32))
 
@@ -778,28 +777,34 @@ def test_a_wait_given_up_is_reported(dev, ops, monkeypatch):
         ops.gated_scan(mine, gate, x, log_gate=True, out=h, final=fin)
 
     def back():
-        ops.gated_scan_backward(mine, gate, h, grad_h, log_gate=True, out=grads)
-    for call, follows in ((scan, mine.sync), (back, mine.sync), (scan, lambda: some.read_array(np.float32))):
-        call()
-        with pytest.raises(hb.EhError, match="in vain"):
-            follows()
-        follows()
-    torch.cuda.synchronize()
-    assert bool(torch.isfinite(h[:, :512]).all()) and bool(torch.isnan(h[:, 512:]).all()) and bool(torch.isnan(fin).all())
-    for follows in (scan, back):                                   # the next scan is not queued
+        ops.gated_scan_backward(mine, gate, x, grad_h, log_gate=True, out=ops.ScanGrads(torch.empty_like(x), h, fin))
+    scan()
+    with pytest.raises(hb.EhError, match="in vain"):
+        mine.sync()
+    mine.sync()
+    assert not bool(h[:, :512].any()) and bool(torch.isnan(h[:, 512:]).all()) and bool(torch.isnan(fin).all())
+    back()
+    with pytest.raises(hb.EhError, match="in vain"):
+        some.read_array(np.float32)
+    some.read_array(np.float32)
+    assert bool(torch.isnan(h[:, :1536]).all()) and bool(torch.isnan(fin).all())
+    for call in (scan, back):                                      # and the next scan is not queued
         scan()
         torch.cuda.synchronize()
         h.zero_()
         with pytest.raises(hb.EhError, match="in vain"):
-            follows()
-        torch.cuda.synchronize()
+            call()
+        mine.sync()
         assert not bool(h.any())
-    dev.sync()                                                       # another handle has lost nothing
+    # another handle has lost nothing, nor does NaN in the data look like a lost wait, whatever its bits
+    x.view(torch.int32)[0, 3, :7] = -1
     ops.gated_scan(dev, gate, x, log_gate=True, out=h, final=fin)
-    want, tol, _, _ = oracle.scan(host(gate), host(x), None, None, True)
-    close(host(h), want, tol, "h")
     dev.sync()
-    mine.sync()
+    assert bool(torch.isnan(fin[0, :7]).all())
+    want, tol, _, _ = oracle.scan(host(gate), np.nan_to_num(host(x)), None, None, True)
+    close(host(h)[..., 7:], want[..., 7:], tol[..., 7:], "h")
+    ops.gated_scan(dev, gate, x, state=x[:, 3].contiguous(), log_gate=True, out=h, final=fin)
+    dev.sync()
 
 
 REFUSED = [
