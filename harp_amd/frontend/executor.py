@@ -128,8 +128,13 @@ def _run_operators(roots: Sequence[GraphNode], input_buffers: Dict[int, object],
         keep.append(memo)
         return out
 
+    def own_view(g: GraphNode) -> GraphNode:
+        return g if g.op.kind != "view" or not g.src else GraphNode([own_view(g.src[0])], g.view, g.op, g.dtype, hint=g.hint)
+
     def dense(g: GraphNode) -> GraphNode:
-        return g if g.view == View.contiguous(g.shape()) and g.op.kind != "view" else g.contiguous()
+        """`g`, copied where it is a view.  The copy reads it through nodes of its own: a view that another node reads too
+        is lowered in another way, with only contiguous ones read right (`lower.rs:209-224`, `:452-455`)."""
+        return g if g.view == View.contiguous(g.shape()) and g.op.kind != "view" else own_view(g).contiguous()
 
     def evaluate(nodes: Sequence[GraphNode]) -> None:
         """Dense buffers for `nodes`, whose graphs have no call left."""

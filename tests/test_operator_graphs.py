@@ -246,6 +246,23 @@ def test_an_operators_source_and_its_views_as_roots(fe):
 
 
 @pytest.mark.parametrize("exact", [True, False])
+def test_a_view_read_by_an_operator_and_by_others(fe, exact):
+    """One strided view as an operator's source, as a root, and inside another source and another root: each has its
+    elements (in both modes, though a view with several readers is lowered differently in them)."""
+    rng = np.random.default_rng(12)
+    a, b = rng.uniform(0.1, 0.9, (2, 4, 3)).astype(np.float32), rng.uniform(0.1, 0.9, (2, 3, 4)).astype(np.float32)
+    with fe.exact_mode(exact):
+        p = tensor(fe, a).permute([0, 2, 1])
+        h = fe.nn.gated_scan(-p, p)
+        q = h.permute([2, 0, 1])
+        got_h, got_q, got_n = many(fe, h, q, -(q * tensor(fe, b.transpose(2, 0, 1).copy())))
+    at = a.transpose(0, 2, 1)
+    want, tol, _, _ = oracle.scan(-at, at, None, None, False)
+    assert np.all(np.abs(got_h - want) <= tol + 2.0 ** -24 * np.abs(want))
+    assert np.array_equal(got_q, got_h.transpose(2, 0, 1)) and np.array_equal(got_n, -(got_h * b).transpose(2, 0, 1))
+
+
+@pytest.mark.parametrize("exact", [True, False])
 def test_gradients_behind_a_reshape_realized_together(fe, exact):
     """The gradients of a step, which are views of one backward call's outputs, from one `realize_many`."""
     rng = np.random.default_rng(9)
