@@ -170,11 +170,11 @@ template <int DT, bool LOG> __device__ inline void step_of(u32x4 vg, u32x4 vx, b
 // pieces, so all are taken.
 //
 // With eight classes, by the workgroup's number, neighbouring columns are read and written behind one
-// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes 31 us
-// instead of 36 (its gradient 50 instead of 60, 64 x 512 x 1000 f32 85 instead of 106).  Where they do start
-// there, one class is better (8 x 4096 x 2048 bf16 88 us instead of 92, the gradient 136 instead of 146).
+// L2: where rows do not start at cache lines they share lines, and 13 x 1999 x 717 f16 takes 37 us
+// instead of 42 (its gradient 65 instead of 71, 64 x 512 x 1000 f32 87 instead of 107).  Where they do start
+// there, one class is better (8 x 4096 x 2048 bf16 89 us instead of 93, the gradient 142 instead of 151).
 //
-// Bound by memory: 8 x 4096 x 2048 bf16 at 4.6 TB/s forward and 4.9 backward, 1 x 131072 x 512 f32 at 5.4.  Smaller
+// Bound by memory: 8 x 4096 x 2048 bf16 at 4.6 TB/s forward and 4.7 backward, 1 x 131072 x 512 f32 at 5.4.  Smaller
 // pieces read the same at more waits and shares of the board, two vectors a lane do not fit the registers.
 template <int DT, int LANES, int W, bool BACK, bool LOG, bool FAR, int EU>
 __global__ __launch_bounds__(64 * W, EU) void scan_pieces(ScanArgs a, int pieces, int tiles, int classes, Board board) {

@@ -428,7 +428,7 @@ template <int THREADS, bool ENT, bool TOP> __global__ __launch_bounds__(THREADS)
 
 // dz_i = c [ g ([i = t] - p_i) - e p_i (log p_i + H) ] with g, e the gradients of log p_t and H: one
 // pass, a vector for each thread.  Workgroups of 4 KB keep what is on the way in memory order:
-// 8192 x 65536 bf16 in 384 us (5.6 TB/s; a copy of as much reaches 5.0); more vectors a thread, or a row for a
+// 8192 x 65536 bf16 in 389 us (5.5 TB/s; a copy of as much reaches 5.0); more vectors a thread, or a row for a
 // workgroup, were 7 and 20% slower.
 template <int DT, bool ENT> __global__ __launch_bounds__(256) void score_grad_rows(ScoreGradArgs a, int spans, int64_t row0) {
   constexpr int N = Elem<DT>::N;

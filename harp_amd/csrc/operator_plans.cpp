@@ -71,8 +71,13 @@ static bool on_lines(const Sequences& s, const ScanArgs& a) {
 // One piece of 16 waves instead of two of 8 with a board: 16 x 700 x 2048 bf16 32 us against 36, 64 x 520 x 1024 57
 // against 64, but many of all 1024 steps 32 x 1000 x 2048 96 against 88 (one workgroup on a compute unit).
 // Wide: one workgroup on a compute unit instead of two, us a gradient with and without, by workgroups of a compute unit:
-//   one    4 x 1999 x 717 f16 19.3 : 20.5       two   4 x 4096 x 1024 bf16 38 : 34, 32 x 512 x 704 f16 27 : 21
-//   eight  8 x 4096 x 2048 bf16 136 : 145       more  64 x 4096 x 1024 bf16 496 : 537, 52 x 2048 x 717 f16 210 : 222
+//   one    4 x 1999 x 717 f16 20.2 : 21.5, 2 x 4096 x 1024 bf16 23.1 : 24.1
+//   two    4 x 4096 x 1024 bf16 49.5 : 49.4, 32 x 512 x 704 f16 34 : 31     three  24 x 512 x 2048 f16 64 : 59
+//   four   32 x 512 x 2048 f16 81 : 80          five  40 x 512 x 2048 f16 98 : 97
+//   six    48 x 512 x 2048 f16 114.6 : 115.3    seven 7 x 4096 x 2048 bf16 128.5 : 129.2
+//   eight  8 x 4096 x 2048 bf16 144 : 147, 64 x 512 x 2048 f16 148 : 151     ten    20 x 4096 x 1024 bf16 174 : 179
+//   more   16 x 4096 x 2048 bf16 261 : 273, 52 x 2048 x 717 f16 215 : 224, 64 x 4096 x 2048 bf16 960 : 1014
+// From two to five it loses or is even, at six and seven the sides differ by less than one in a hundred.
 // (in f32, which needs fewer registers, 161 : 156 and 497 : 502)
 ScanPlan plan_scan(const ScanArgs& a) {
   ScanPlan p{};

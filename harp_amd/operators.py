@@ -16,6 +16,10 @@ that this library works on, `HipDevice(index, stream=...)`.
     grad = token_logprobs_backward(dev, logits, targets, norm, entropy, grad_logp, grad_entropy, out=grad)
 
 Without `out` the results are new `HipBuffer`s.  Nothing waits for the GPU.
+
+Tensors of another library are memory to these calls: none of them is recorded for that library's differentiation
+(a tensor that requires a gradient is read like any other, and gets none from here; each call's gradient is its `_backward`),
+and what is written to `out` is not counted as a change of it.  The calls do not keep a tensor alive for work that is queued.
 """
 
 from __future__ import annotations
@@ -274,7 +278,8 @@ def gated_scan(device: HipDevice, gate, x, *, state=None, lengths=None, log_gate
                workspace=None):
     """h_t = a_t h_(t-1) + x_t along axis 1 of [batch, time, width], with a = gate or exp(gate); h_(-1) is `state`
     [batch, width] (f32) or 0.  `final` receives h of the last step in f32: the next call's `state`, which makes a call
-    with time 1 a decoding step.  `lengths` [batch] (i32): steps behind them are neither read nor written.  Returns `out`."""
+    with time 1 a decoding step.  `lengths` [batch] (i32): steps behind them are neither read nor written, so that `out` holds there what it held (a new one:
+    zeros).  Returns `out`."""
     shape, code, g = _array(device, gate, "gate", 3)
     shape = tuple(shape)
     batch, time, width = shape
